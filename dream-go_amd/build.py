@@ -11,7 +11,10 @@
                               board kernels, the stamp / trace hooks -- and every test entry.  Its tests: tests/ablations/ (collected only
                               when that library is the one loaded, DGNN_LIBRARY=dream-go_amd/lib/ablations/libdgnn_hip.so)
 
-Both depend only on the HIP runtime (libamdhip64); neither links torch.
+    lib/libdgnn_ops.so        the operators on device tensors (include/dgnn_ops.h), a library of its own: a predictor that is not the
+                              reference's network is put together from them, and a host that runs the engine alone does not load them
+
+All depend only on the HIP runtime (libamdhip64); none links torch.
 """
 import os
 import subprocess
@@ -27,6 +30,11 @@ TEST_LIB_PATH = LIB_PATH if ABLATIONS else os.path.join(LIB_DIR, "libdgnn_hip_te
 
 HOST_SOURCES = ["loader.cpp", "network.cpp", "engine.cpp", "rccl.cpp", "batcher.cpp", "formats.cpp", "tree.cpp", "search.cpp", "go.cpp", "fiber.cpp"]
 KERNEL_SOURCES = ["conv_board.hip", "conv_board_b.hip", "conv_board_tower.hip", "kernels.hip", "heads.hip", "features.hip"]
+OPS_LIB_PATH = os.path.join(HERE, "lib", "libdgnn_ops.so")
+OPS_SOURCES = ["ops.cpp", "ops_dense.hip", "ops_group_norm.hip", "ops_logits.hip"]
+# The operators' kernels use no packed fp32 arithmetic: the compiler forms v_pk_{add,mul,fma}_f32 from plain float code, and some forms
+# have given wrong results on this part.  (The host pass does not know the feature and says so.)
+OPS_FLAGS = ["-fvisibility=hidden", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-result"]
 if ABLATIONS:
     FLAGS.append("-DDGNN_ABLATIONS")
@@ -51,7 +59,7 @@ def _stamp():
         version = subprocess.run([hipcc(), "--version"], capture_output=True, text=True, timeout=60).stdout.strip().splitlines()[0]
     except Exception:   # noqa: BLE001
         version = "unknown hipcc"
-    return " ".join(FLAGS + LINK_FLAGS) + "\n" + version + "\n"
+    return " ".join(FLAGS + LINK_FLAGS + OPS_FLAGS) + "\n" + version + "\n"
 
 
 def _stamp_matches():
@@ -69,14 +77,20 @@ def _headers():
 def _kernel_headers():
     """The kernel translation units include the csrc headers only (kernels.h, conv_board_body.h ...), never the public ones: a change of
     include/*.h recompiles the host sources (seconds), not the kernels (minutes)."""
-    return [os.path.join(CSRC, n) for n in os.listdir(CSRC) if n.endswith(".h") and n != "dgnn_internal.h"]
+    return [os.path.join(CSRC, n) for n in os.listdir(CSRC) if n.endswith(".h") and n not in ("dgnn_internal.h", "ops.h", "ops_device.h")]
+
+
+def _ops_headers():
+    inc = os.path.join(HERE, "..", "include")
+    return [os.path.join(CSRC, n) for n in ("ops.h", "ops_device.h")] + [os.path.join(inc, n) for n in ("dgnn.h", "dgnn_ops.h")]
 
 
 def needs_build():
-    if not os.path.exists(LIB_PATH) or not os.path.exists(TEST_LIB_PATH) or not _stamp_matches():
+    libraries = [LIB_PATH, TEST_LIB_PATH] + ([] if ABLATIONS else [OPS_LIB_PATH])
+    if not all(os.path.exists(p) for p in libraries) or not _stamp_matches():
         return True
-    built = min(os.path.getmtime(LIB_PATH), os.path.getmtime(TEST_LIB_PATH))
-    return any(os.path.getmtime(d) > built for d in _headers() + [os.path.join(CSRC, n) for n in HOST_SOURCES + KERNEL_SOURCES])
+    built = min(os.path.getmtime(p) for p in libraries)
+    return any(os.path.getmtime(d) > built for d in _headers() + [os.path.join(CSRC, n) for n in HOST_SOURCES + KERNEL_SOURCES + OPS_SOURCES])
 
 
 def _stale(src_path, obj, headers):
@@ -97,7 +111,7 @@ def build(force=False, verbose=False):
         if os.path.exists(stale):
             os.remove(stale)
     jobs, running = [], []
-    kernel_objects, host_objects, test_objects = [], [], []
+    kernel_objects, host_objects, test_objects, ops_objects = [], [], [], []
     for src in KERNEL_SOURCES:
         obj = os.path.join(LIB_DIR, os.path.basename(src).rsplit(".", 1)[0] + ".o")
         kernel_objects.append(obj)
@@ -110,6 +124,11 @@ def build(force=False, verbose=False):
             tobj = os.path.join(LIB_DIR, "test", src.rsplit(".", 1)[0] + ".o")
             test_objects.append(tobj)
             jobs.append((src, tobj, ["-DDGNN_TEST_ENTRIES"], _headers()))
+    if not ABLATIONS:
+        for src in OPS_SOURCES:
+            obj = os.path.join(LIB_DIR, src.rsplit(".", 1)[0] + ".o")
+            ops_objects.append(obj)
+            jobs.append((src, obj, OPS_FLAGS, _ops_headers()))
     # The translation units are independent: compile them side by side, as many at a time as there are CPUs, the kernel units (the
     # long ones: the critical path of a clean build) first, so that they never share a core with the twenty short host units.
     pending = []
@@ -138,6 +157,7 @@ def build(force=False, verbose=False):
     links = [(LIB_PATH, host_objects + kernel_objects)]
     if not ABLATIONS:
         links.append((TEST_LIB_PATH, test_objects + kernel_objects))
+        links.append((OPS_LIB_PATH, ops_objects))
     for path, objects in links:
         cmd = [hipcc(), *LINK_FLAGS, "-o", path, *objects]
         if verbose:
