@@ -38,14 +38,61 @@ __device__ __forceinline__ float load_either(const void* p, int64_t i, bool is_f
     return is_float ? static_cast<const float*>(p)[i] : (float)static_cast<const T*>(p)[i];
 }
 
+__device__ __forceinline__ float rcp(float v) { return __builtin_amdgcn_rcpf(v); }                          // one step off at most
+__device__ __forceinline__ float exponential(float v) { return __builtin_amdgcn_exp2f(v * 1.44269504088896341f); }
+
+// The activations in fp32, without branches: a wave does eight of them per lane in a row.  Errors are a few steps of fp32 beside max(1, |v|).
+//   tanh  its series (to x^11) up to 1/4, 1 - 2 / (exp(2 x) + 1) beyond, where nothing cancels
+//   gelu  v * Phi(v) with erfc from Abramowitz & Stegun 7.1.26 (absolute error 1.5e-7); the tail is the product itself, not 1 - erf
+__device__ __forceinline__ float tanh_of(float v)
+{
+    const float q = v * v;
+    const float series = v * __builtin_fmaf(q, __builtin_fmaf(q, __builtin_fmaf(q, __builtin_fmaf(q, __builtin_fmaf(q, -8.86323553e-3f, 2.18694885e-2f),
+                             -5.39682540e-2f), 1.33333333e-1f), -3.33333333e-1f), 1.0f);
+    const float direct = 1.0f - 2.0f * rcp(exponential(2.0f * v) + 1.0f);
+    return __builtin_fabsf(v) < 0.25f ? series : direct;
+}
+__device__ __forceinline__ float gelu_of(float v)
+{
+    const float x = __builtin_fabsf(v) * 0.70710678118654752f, t = rcp(__builtin_fmaf(0.3275911f, x, 1.0f));
+    const float p = t * __builtin_fmaf(t, __builtin_fmaf(t, __builtin_fmaf(t, __builtin_fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+    const float tail = 0.5f * p * exponential(-x * x);           // Phi(-|v|)
+    return v * (v < 0.0f ? tail : 1.0f - tail);
+}
+__device__ __forceinline__ float silu_of(float v) { return v * rcp(1.0f + exponential(-v)); }
+
 __device__ __forceinline__ float activate(float v, int activation)
 {
     switch (activation) {
     case DGNN_ACT_RELU: return v < 0.0f ? 0.0f : v;
-    case DGNN_ACT_TANH: return tanhf(v);
-    case DGNN_ACT_GELU: return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
-    case DGNN_ACT_SILU: return v / (1.0f + expf(-v));
+    case DGNN_ACT_TANH: return tanh_of(v);
+    case DGNN_ACT_GELU: return gelu_of(v);
+    case DGNN_ACT_SILU: return silu_of(v);
     default: return v;
+    }
+}
+
+// One branch for several values.
+template <int N>
+__device__ __forceinline__ void activate(float (&v)[N], int activation)
+{
+    switch (activation) {
+    case DGNN_ACT_IDENTITY: break;
+    case DGNN_ACT_RELU:
+#pragma unroll
+        for (int r = 0; r < N; ++r) v[r] = activate(v[r], DGNN_ACT_RELU);
+        break;
+    case DGNN_ACT_TANH:
+#pragma unroll
+        for (int r = 0; r < N; ++r) v[r] = activate(v[r], DGNN_ACT_TANH);
+        break;
+    case DGNN_ACT_GELU:
+#pragma unroll
+        for (int r = 0; r < N; ++r) v[r] = activate(v[r], DGNN_ACT_GELU);
+        break;
+    default:
+#pragma unroll
+        for (int r = 0; r < N; ++r) v[r] = activate(v[r], DGNN_ACT_SILU);
     }
 }
 
