@@ -27,6 +27,14 @@ __device__ __forceinline__ void mfma_tied(vec<T, 8> a, vec<T, 8> b, floatx4& c)
 }
 __device__ __forceinline__ void settle() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
 
+// Everything asked for has arrived; the builtin, so that the compiler knows too.
+__device__ __forceinline__ void wait_all()
+{
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070);         // vmcnt(0) expcnt(7) lgkmcnt(0)
+    asm volatile("" ::: "memory");
+}
+
 // Up to eight neighbouring outputs of row m, from column n on: everything behind the sums.
 template <typename T, typename O>
 __device__ __forceinline__ void finish_as(const dgnn_dense_args& a, int64_t m, int64_t n, float (&v)[8])
@@ -118,18 +126,19 @@ struct Tile {
     static constexpr int kLoadsW = BN / 8 / kWaves;
     static_assert(BN / 8 % kWaves == 0 && BM / 8 % kWaves == 0, "whole pieces");
     static constexpr int kReads = FN + FM, kProducts = FN * FM;
-    static constexpr bool kTied = FN * FM == 64;
+    static constexpr bool kTied = FN * FM >= 32;
     typedef vec<T, 8> Frag;
 
     struct Frags { Frag w[FN], x[FM]; };
 
     const dgnn_dense_args& a;
     T* const lds;                                               // [2][kRows][64]
-    const int lane, wave;
+    int lane;
+    const int wave;
     const int64_t m0, n0;
-    unsigned offset[kLoads];                                    // DMA: bytes from the tile's first row of W (x) to this lane's segment
     const char* base_w;
     const char* base_x;
+    int last_w, last_x;                                         // the last row of the tile's W (x) that is there
     int read_w, read_x;                                         // elements: this lane's row of fragment 0, and its segment of step 0 and 1
     int seg[2];
     vec<T, 8> staged[DMA ? 1 : kLoads];
@@ -139,10 +148,8 @@ struct Tile {
     {
         base_w = static_cast<const char*>(a.w) + n0 * a.ldw * 2;
         base_x = static_cast<const char*>(a.x) + m0 * a.ldx * 2;
-        if constexpr (DMA) {
-#pragma unroll
-            for (int j = 0; j < kLoads; ++j) offset[j] = (unsigned)(row_of(j) * (j < kLoadsW ? a.ldw : a.ldx) * 2 + segment_of(j) * 16);
-        }
+        last_w = (int)(a.n - n0 < BN ? a.n - n0 : BN) - 1;
+        last_x = (int)(a.m - m0 < BM ? a.m - m0 : BM) - 1;
         const int r = lane & 15;
         read_w = ((wave % WN) * FN * 16 + r) * BK;
         read_x = (BN + (wave / WN) * FM * 16 + r) * BK;
@@ -150,15 +157,15 @@ struct Tile {
         for (int s = 0; s < 2; ++s) seg[s] = ((s * 4 + (lane >> 4)) ^ (r >> 1 & 7)) * 8;
     }
 
-    // piece j of this wave: which row of the tile's W (x) this lane fetches -- beyond the last row that one again, its outputs are never stored --
-    // and which of its segments
+    // Piece j of this wave: which row of the tile's W (x) this lane fetches -- beyond the last row that one again, its outputs are never stored --
+    // and which of its segments.
     __device__ __forceinline__ int piece(int j) const { return j < kLoadsW ? wave * kLoadsW + j : BN / 8 + wave * (kLoads - kLoadsW) + j - kLoadsW; }
-    __device__ __forceinline__ int64_t row_of(int j) const
+    __device__ __forceinline__ int row_of(int j) const
     {
-        const int64_t row = piece(j) * 8 + (lane >> 3) - (j < kLoadsW ? 0 : BN), rows = j < kLoadsW ? a.n - n0 : a.m - m0;
-        return row < rows ? row : rows - 1;
+        const int row = (j < kLoadsW ? piece(j) : piece(j) - BN / 8) * 8 + (lane >> 3), last = j < kLoadsW ? last_w : last_x;
+        return row < last ? row : last;
     }
-    __device__ __forceinline__ int segment_of(int j) const { return (lane & 7) ^ ((piece(j) * 8 + (lane >> 3)) >> 1 & 7); }
+    __device__ __forceinline__ int segment_of(int j) const { return (lane & 7) ^ ((piece(j) * 4 + (lane >> 4)) & 7); }
 
     __device__ __forceinline__ const T* source(int j, int64_t k) const
     {
@@ -174,12 +181,16 @@ struct Tile {
 #pragma unroll
         for (int j = 0; j < kLoads; ++j) write(j, buffer, load_row<T>(source(j, 0), k + segment_of(j) * 8, a.k));
     }
-    __device__ __forceinline__ void load(int j, int buffer, int64_t k)
+    // Piece j of the tile whose first column is at `w` (`x`) in the tile's first row.  The offset of a row is a 24-bit product, formed anew each time:
+    // kept, the offsets of all pieces would be more registers than the sums leave.
+    __device__ __forceinline__ void load(int j, int buffer, const char* w, const char* x)
     {
         if constexpr (DMA) {
-            dma_row((j < kLoadsW ? base_w : base_x) + k * 2, offset[j], lds + buffer * kRows * BK + piece(j) * 8 * BK);
+            const unsigned offset = __umul24(row_of(j), (unsigned)(j < kLoadsW ? a.ldw : a.ldx) * 2) + segment_of(j) * 16;
+            dma_row(j < kLoadsW ? w : x, offset, lds + buffer * kRows * BK + piece(j) * 8 * BK);
         } else {
-            staged[j] = load_vec<T, 8>(source(j, k + segment_of(j) * 8));
+            const T* const row = reinterpret_cast<const T*>(j < kLoadsW ? w : x) + row_of(j) * (j < kLoadsW ? a.ldw : a.ldx);
+            staged[j] = load_vec<T, 8>(row + segment_of(j) * 8);
         }
     }
     __device__ __forceinline__ void read(int r, int buffer, int step, Frags& f) const
@@ -193,69 +204,74 @@ struct Tile {
     // The products of one step; beside them the fragments of the next step are read and, with LOAD, the tile two ahead is asked for.  Nothing in
     // here branches: the compiler keeps the sums and the fragments where they are.
     template <bool LOAD>
-    __device__ __forceinline__ void step(floatx4 (&acc)[FN][FM], const Frags& f, Frags& next, int read_buffer, int read_step, int load_buffer, int64_t k)
+    __device__ __forceinline__ void step(floatx4 (&acc)[FN][FM], const Frags& f, Frags& next, int read_buffer, int read_step, int load_buffer, const char* w, const char* x)
     {
-        constexpr int kGroups = kReads;
+        constexpr int kGroups = kReads, kReadGroups = kGroups * 3 / 4;
 #pragma unroll
         for (int g = 0; g < kGroups; ++g) {
-            if constexpr (LOAD) {
-#pragma unroll
-                for (int j = g * kLoads / kGroups; j < (g + 1) * kLoads / kGroups; ++j) load(j, load_buffer, k);
-            }
-            read(g, read_buffer, read_step, next);
 #pragma unroll
             for (int p = g * kProducts / kGroups; p < (g + 1) * kProducts / kGroups; ++p)
                 if constexpr (kTied) mfma_tied<T>(f.w[p / FM], f.x[p % FM], acc[p / FM][p % FM]);
                 else acc[p / FM][p % FM] = mfma<T>(f.w[p / FM], f.x[p % FM], acc[p / FM][p % FM]);
+            if constexpr (LOAD) {
+#pragma unroll
+                for (int j = g * kLoads / kGroups; j < (g + 1) * kLoads / kGroups; ++j) load(j, load_buffer, w, x);
+            }
+            if (g < kReadGroups) {
+#pragma unroll
+                for (int r = g * kReads / kReadGroups; r < (g + 1) * kReads / kReadGroups; ++r) read(r, read_buffer, read_step, next);
+            }
             __builtin_amdgcn_sched_barrier(0);
         }
     }
 
     // Tile t, whose first fragments are in f0; leaves those of tile t + 1 there (behind the last tile: whatever the buffer holds).
     template <bool LOAD>
-    __device__ __forceinline__ void tile(floatx4 (&acc)[FN][FM], Frags& f0, Frags& f1, int64_t t, int64_t k)
+    __device__ __forceinline__ void tile(floatx4 (&acc)[FN][FM], Frags& f0, Frags& f1, int t, int k)
     {
-        const int b = (int)(t & 1);
-        step<false>(acc, f0, f1, b, 1, 0, 0);
+        const int b = t & 1;
+        step<false>(acc, f0, f1, b, 1, 0, nullptr, nullptr);
         if constexpr (!DMA) {
             if (t > 0) {
 #pragma unroll
                 for (int j = 0; j < kLoads; ++j) write(j, b ^ 1, staged[j]);
             }
         }
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        wait_all();
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        step<LOAD>(acc, f1, f0, b ^ 1, 0, b, k);
+        const char *w = base_w + (int64_t)k * 2, *x = base_x + (int64_t)k * 2;
+        asm volatile("" : "+s"(w), "+s"(x), "+v"(lane));        // (otherwise every piece's address is kept in registers and counted up)
+        step<LOAD>(acc, f1, f0, b ^ 1, 0, b, w, x);
     }
 
     __device__ __forceinline__ void run(floatx4 (&acc)[FN][FM])
     {
-        const int64_t whole = a.k / BK, ragged = a.k % BK ? 1 : 0, tiles = whole + ragged;
+        const int whole = (int)(a.k / BK), ragged = a.k % BK ? 1 : 0, tiles = whole + ragged;
         if (tiles == 0) return;
         // tile t starts at column first + t * 64, the ragged one (t = 0) at the end of the row
-        const int64_t first = ragged ? -BK : 0;
+        const int first = ragged ? -BK : 0;
         __syncthreads();                                        // (the LDS of the tile before)
-        if (ragged) load_ragged(0, whole * BK);
+        if (ragged) load_ragged(0, (int64_t)whole * BK);
         else fill(0, 0);
         if (tiles > 1) fill(1, first + BK);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        wait_all();
         __syncthreads();
         Frags f0, f1;
 #pragma unroll
         for (int r = 0; r < kReads; ++r) read(r, 0, 0, f0);
-        int64_t t = 0;
+        int t = 0;
         for (; t + 2 < tiles; ++t) tile<true>(acc, f0, f1, t, first + (t + 2) * BK);
         for (; t < tiles; ++t) tile<false>(acc, f0, f1, t, 0);
         if constexpr (kTied) settle();
     }
 
     // a whole tile, at once (before the loop)
-    __device__ __forceinline__ void fill(int buffer, int64_t k)
+    __device__ __forceinline__ void fill(int buffer, int k)
     {
 #pragma unroll
         for (int j = 0; j < kLoads; ++j) {
-            load(j, buffer, k);
+            load(j, buffer, base_w + (int64_t)k * 2, base_x + (int64_t)k * 2);
             if constexpr (!DMA) write(j, buffer, staged[j]);
         }
     }
@@ -310,7 +326,7 @@ __device__ __forceinline__ void place(int64_t i, int64_t tiles_m, int64_t tiles_
 }
 
 template <typename T, int FN, int FM, int WN, int WM, bool DMA>
-__global__ __launch_bounds__(WN * WM * 64, FN * FM > 16 ? 1 : 2)
+__global__ __launch_bounds__(WN * WM * 64, FN * FM > 32 ? 1 : 2)
 void dense_tile_kernel(dgnn_dense_args a, int64_t tiles_m, int64_t tiles_n)
 {
     typedef Tile<T, FN, FM, WN, WM, DMA> Work;
@@ -342,7 +358,7 @@ hipError_t launch_typed(const dgnn_dense_args& a, hipStream_t stream)
     const bool dma = sixteen(a.x, a.ldx, a.m) && sixteen(a.w, a.ldw, a.n) && a.ldx < 1 << 22 && a.ldw < 1 << 22;
     if (!dma) return launch_tiles<T, 4, 4, 2, 2, false>(a, stream);
     const int64_t big = ((a.m + 255) / 256) * ((a.n + 255) / 256);
-    if (big >= 192) return launch_tiles<T, 8, 8, 2, 2, true>(a, stream);
+    if (big >= 192) return launch_tiles<T, 4, 8, 4, 2, true>(a, stream);
     const int64_t mid = ((a.m + 127) / 128) * ((a.n + 127) / 128);
     if (mid >= 128) return launch_tiles<T, 4, 4, 2, 2, true>(a, stream);
     return launch_tiles<T, 2, 2, 2, 2, true>(a, stream);
