@@ -53,6 +53,8 @@ bool aligned(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(
 bool float_type(int32_t t) { return t == DGNN_F16 || t == DGNN_BF16 || t == DGNN_F32; }
 bool activation_ok(int32_t a) { return a >= DGNN_ACT_IDENTITY && a <= DGNN_ACT_SILU; }
 
+bool holds(const void* workspace, int64_t bytes, int64_t need) { return need == 0 || (workspace && bytes >= need && aligned(workspace, 256)); }
+
 // rows of `width` bytes, `pitch` bytes apart
 struct Rows {
     const void* data;
@@ -181,10 +183,21 @@ extern "C" {
 
 __attribute__((visibility("default"))) int dgnn_ops_last_hip_error(void) { return g_last_hip_error; }
 
+__attribute__((visibility("default"))) int dgnn_dense_workspace(const dgnn_dense_args* args, int64_t* bytes)
+{
+    if (!bytes) return DGNN_BAD_ARGUMENT;
+    *bytes = 0;
+    const int status = check(args);
+    if (status != DGNN_OK || args->m == 0 || args->n == 0) return status;
+    *bytes = dgnn::ops::dense_workspace(*args);
+    return DGNN_OK;
+}
+
 __attribute__((visibility("default"))) int dgnn_dense(int device, void* hip_stream, const dgnn_dense_args* args)
 {
     const int status = check(args);
     if (status != DGNN_OK || args->m == 0 || args->n == 0) return status;
+    if (!holds(args->workspace, args->workspace_bytes, dgnn::ops::dense_workspace(*args))) return DGNN_BAD_ARGUMENT;
     return run(device, hip_stream, *args, dgnn::ops::launch_dense);
 }
 
@@ -202,8 +215,7 @@ __attribute__((visibility("default"))) int dgnn_group_norm(int device, void* hip
 {
     const int status = check(args);
     if (status != DGNN_OK || args->n == 0 || args->p == 0 || args->c == 0) return status;
-    const int64_t need = dgnn::ops::group_norm_workspace(*args);
-    if (need > 0 && (!args->workspace || args->workspace_bytes < need || !aligned(args->workspace, 16))) return DGNN_BAD_ARGUMENT;
+    if (!holds(args->workspace, args->workspace_bytes, dgnn::ops::group_norm_workspace(*args))) return DGNN_BAD_ARGUMENT;
     return run(device, hip_stream, *args, dgnn::ops::launch_group_norm);
 }
 

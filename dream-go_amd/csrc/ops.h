@@ -9,17 +9,22 @@ namespace dgnn {
 namespace ops {
 
 // Launches `kernel` and returns what the launch itself said (hipGetLastError would also return, and clear, what others left there).
+template <typename... Params>
+hipError_t launch_as(void (*kernel)(Params...), dim3 grid, dim3 block, hipStream_t stream, Params... args)
+{
+    void* pointers[] = {const_cast<void*>(static_cast<const void*>(&args))...};
+    return hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, block, pointers, 0, stream);
+}
 template <typename... Params, typename... Args>
 hipError_t launch(void (*kernel)(Params...), dim3 grid, dim3 block, hipStream_t stream, Args... args)
 {
-    static_assert(sizeof...(Params) == sizeof...(Args), "one argument per parameter");
-    void* pointers[] = {static_cast<void*>(&args)...};
-    return hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, block, pointers, 0, stream);
+    return launch_as<Params...>(kernel, grid, block, stream, args...);
 }
 
 // A grid dimension times the workgroup's has to stay below 2^32; kernels loop over what a capped grid leaves.
 constexpr int64_t kMaxGrid = 1 << 20;
 
+int64_t dense_workspace(const dgnn_dense_args& a);
 hipError_t launch_dense(const dgnn_dense_args& a, hipStream_t stream);
 int64_t group_norm_workspace(const dgnn_group_norm_args& a);
 hipError_t launch_group_norm(const dgnn_group_norm_args& a, hipStream_t stream);

@@ -27,11 +27,13 @@ __device__ __forceinline__ void mfma_tied(vec<T, 8> a, vec<T, 8> b, floatx4& c)
 }
 __device__ __forceinline__ void settle() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
 
-// Everything asked for has arrived; the builtin, so that the compiler knows too.
-__device__ __forceinline__ void wait_all()
+// Every LDS operation of the wave is done and at most N of its loads are still on their way; the builtin, so that the compiler knows too.
+template <int N>
+__device__ __forceinline__ void wait_for_all_but()
 {
+    static_assert(N < 64, "the counter has six bits");
     asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0x0070);         // vmcnt(0) expcnt(7) lgkmcnt(0)
+    __builtin_amdgcn_s_waitcnt((N & 15) | 0x0070 | (N >> 4) << 14);             // vmcnt(N) expcnt(7) lgkmcnt(0)
     asm volatile("" ::: "memory");
 }
 
@@ -39,6 +41,8 @@ __device__ __forceinline__ void wait_all()
 template <typename T, typename O>
 __device__ __forceinline__ void finish_as(const dgnn_dense_args& a, int64_t m, int64_t n, float (&v)[8])
 {
+#pragma unroll
+    for (int r = 0; r < 8; ++r) v[r] *= a.alpha1;
     const O* const z = a.z ? static_cast<const O*>(a.z) + m * a.ldz + n : nullptr;
     O* const y = static_cast<O*>(a.y) + m * a.ldy + n;
     const bool bias_is_float = a.bias_type == DGNN_F32;
@@ -87,6 +91,23 @@ __device__ __forceinline__ void finish(const dgnn_dense_args& a, int64_t m, int6
     else finish_as<T, T>(a, m, n, v);
 }
 
+// The sums of one share of k, as they are: dense_join_kernel finishes them.
+__device__ __forceinline__ void keep(const dgnn_dense_args& a, float* part, int64_t m, int64_t n, const float (&v)[8])
+{
+    if (m >= a.m || n >= a.n) return;
+    float* const to = part + m * a.n + n;
+    if (n + 8 <= a.n) {
+        vec<float, 8> all;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) all[r] = v[r];
+        store_vec<float, 8>(to, all);
+    } else {
+#pragma unroll
+        for (int r = 0; r < 7; ++r)
+            if (n + r < a.n) to[r] = v[r];
+    }
+}
+
 // Eight elements of a row from column k on; zero at and beyond `k_end`.
 template <typename T>
 __device__ __forceinline__ vec<T, 8> load_row(const T* row, int64_t k, int64_t k_end)
@@ -107,47 +128,50 @@ __device__ __forceinline__ void dma_row(const char* base, unsigned offset, T* ld
 
 // ---- tiles through LDS ------------------------------------------------------------------------------------------------------------
 //
-// WN x WM waves, each FN x FM fragments of 16 x 16 outputs; 64 of k at a time, double buffered.  A row's 64 elements are 128 bytes of LDS,
+// WN x WM waves, each FN x FM fragments of 16 x 16 outputs; 64 of k at a time in a ring of S tiles.  A row's 64 elements are 128 bytes of LDS,
 // its eight 16-byte segments stored at position segment ^ (row / 2 % 8): the sixteen lanes that one ds_read_b128 cycle serves (0-3, 12-15,
 // 20-27 and the like: two segments, eight rows each) then fall into sixteen different 16-byte columns of the 64 banks.
 //
 // A tile is two steps of k = 32.  While the products of one step run, the fragments of the next are read, so a wave never waits for the read
 // it has just asked for; the buffer of a tile is free once its second step has been read, i.e. at the one barrier in the middle of each tile,
-// and is filled again two tiles ahead: a load has a whole tile's products to arrive.
-//   DMA    rows whose address and stride are multiples of 16 bytes go from memory into LDS without passing through registers
-//   else   the same pipeline with loads into registers (unaligned, but as wide) and ds_writes one tile later
-// What is left of k behind the last whole tile (masked, element by element) comes FIRST: it is the one tile that is always written through registers.
-template <typename T, int FN, int FM, int WN, int WM, bool DMA>
+// and is filled again S tiles ahead: a load has S - 1 tiles' products to arrive, and is waited for by count.
+// Rows go from memory into LDS without passing through registers: their addresses and strides are multiples of 16 bytes (dense_pack_kernel sees
+// to it where the caller's are not).  What is left of k behind the last whole tile (masked, element by element) comes FIRST: it is the one tile
+// that is written through registers.
+template <typename T, int FN, int FM, int WN, int WM, int S>
 struct Tile {
     static constexpr int kWaves = WN * WM, kThreads = kWaves * 64;
     static constexpr int BN = WN * FN * 16, BM = WM * FM * 16, BK = 64;
     static constexpr int kRows = BN + BM;
-    static constexpr int kLoads = kRows / 8 / kWaves;           // 1 KiB pieces (8 rows) per wave and tile: first those of W, then those of x
-    static constexpr int kLoadsW = BN / 8 / kWaves;
-    static_assert(BN / 8 % kWaves == 0 && BM / 8 % kWaves == 0, "whole pieces");
+    static constexpr int kPieces = kRows / 8, kPiecesW = BN / 8;                // 1 KiB pieces (8 rows): first those of W, then those of x
+    static constexpr bool kEven = kPiecesW % kWaves == 0 && kPieces % kWaves == 0;
+    static constexpr int kLoads = (kPieces + kWaves - 1) / kWaves, kLoadsW = kEven ? kPiecesW / kWaves : 0;
     static constexpr int kReads = FN + FM, kProducts = FN * FM;
     static constexpr bool kTied = FN * FM >= 32;
+    static constexpr int kLdsBytes = S * kRows * BK * 2;
+    static constexpr int kPerUnit = 160 * 1024 / kLdsBytes < 2 ? 1 : 2;         // workgroups on a compute unit at a time
+    static_assert(S >= 2 && (S - 2) * kLoads < 64, "loads in flight are counted");
     typedef vec<T, 8> Frag;
 
     struct Frags { Frag w[FN], x[FM]; };
 
     const dgnn_dense_args& a;
-    T* const lds;                                               // [2][kRows][64]
+    T* const lds;                                               // [S][kRows][64]
     int lane;
     const int wave;
     const int64_t m0, n0;
+    const int columns;                                          // of k, from `begin` on
     const char* base_w;
     const char* base_x;
     int last_w, last_x;                                         // the last row of the tile's W (x) that is there
     int read_w, read_x;                                         // elements: this lane's row of fragment 0, and its segment of step 0 and 1
     int seg[2];
-    vec<T, 8> staged[DMA ? 1 : kLoads];
 
-    __device__ __forceinline__ Tile(const dgnn_dense_args& args, T* memory, int64_t m, int64_t n)
-        : a(args), lds(memory), lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), m0(m), n0(n)
+    __device__ __forceinline__ Tile(const dgnn_dense_args& args, T* memory, int64_t m, int64_t n, int64_t begin, int64_t end)
+        : a(args), lds(memory), lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), m0(m), n0(n), columns((int)(end - begin))
     {
-        base_w = static_cast<const char*>(a.w) + n0 * a.ldw * 2;
-        base_x = static_cast<const char*>(a.x) + m0 * a.ldx * 2;
+        base_w = static_cast<const char*>(a.w) + (n0 * a.ldw + begin) * 2;
+        base_x = static_cast<const char*>(a.x) + (m0 * a.ldx + begin) * 2;
         last_w = (int)(a.n - n0 < BN ? a.n - n0 : BN) - 1;
         last_x = (int)(a.m - m0 < BM ? a.m - m0 : BM) - 1;
         const int r = lane & 15;
@@ -158,40 +182,44 @@ struct Tile {
     }
 
     // Piece j of this wave: which row of the tile's W (x) this lane fetches -- beyond the last row that one again, its outputs are never stored --
-    // and which of its segments.
-    __device__ __forceinline__ int piece(int j) const { return j < kLoadsW ? wave * kLoadsW + j : BN / 8 + wave * (kLoads - kLoadsW) + j - kLoadsW; }
+    // and which of its segments.  Where the pieces do not divide evenly the last one is fetched more than once, by every wave alike many loads.
+    __device__ __forceinline__ int piece(int j) const
+    {
+        if constexpr (kEven) return j < kLoadsW ? wave * kLoadsW + j : kPiecesW + wave * (kLoads - kLoadsW) + j - kLoadsW;
+        else return wave * kLoads + j < kPieces ? wave * kLoads + j : kPieces - 1;
+    }
+    __device__ __forceinline__ bool of_w(int j) const
+    {
+        if constexpr (kEven) return j < kLoadsW;
+        else return piece(j) < kPiecesW;
+    }
     __device__ __forceinline__ int row_of(int j) const
     {
-        const int row = (j < kLoadsW ? piece(j) : piece(j) - BN / 8) * 8 + (lane >> 3), last = j < kLoadsW ? last_w : last_x;
+        const int row = (of_w(j) ? piece(j) : piece(j) - kPiecesW) * 8 + (lane >> 3), last = of_w(j) ? last_w : last_x;
         return row < last ? row : last;
     }
     __device__ __forceinline__ int segment_of(int j) const { return (lane & 7) ^ ((piece(j) * 4 + (lane >> 4)) & 7); }
 
-    __device__ __forceinline__ const T* source(int j, int64_t k) const
+    __device__ __forceinline__ const T* source(int j) const
     {
-        return reinterpret_cast<const T*>(j < kLoadsW ? base_w : base_x) + row_of(j) * (j < kLoadsW ? a.ldw : a.ldx) + k;
+        return reinterpret_cast<const T*>(of_w(j) ? base_w : base_x) + row_of(j) * (of_w(j) ? a.ldw : a.ldx);
     }
     __device__ __forceinline__ void write(int j, int buffer, Frag v)
     {
         *reinterpret_cast<Frag*>(lds + buffer * kRows * BK + piece(j) * 8 * BK + lane * 8) = v;
     }
     // the ragged piece of k, through registers
-    __device__ __forceinline__ void load_ragged(int buffer, int64_t k)
+    __device__ __forceinline__ void load_ragged(int buffer, int k)
     {
 #pragma unroll
-        for (int j = 0; j < kLoads; ++j) write(j, buffer, load_row<T>(source(j, 0), k + segment_of(j) * 8, a.k));
+        for (int j = 0; j < kLoads; ++j) write(j, buffer, load_row<T>(source(j), k + segment_of(j) * 8, columns));
     }
     // Piece j of the tile whose first column is at `w` (`x`) in the tile's first row.  The offset of a row is a 24-bit product, formed anew each time:
     // kept, the offsets of all pieces would be more registers than the sums leave.
     __device__ __forceinline__ void load(int j, int buffer, const char* w, const char* x)
     {
-        if constexpr (DMA) {
-            const unsigned offset = __umul24(row_of(j), (unsigned)(j < kLoadsW ? a.ldw : a.ldx) * 2) + segment_of(j) * 16;
-            dma_row(j < kLoadsW ? w : x, offset, lds + buffer * kRows * BK + piece(j) * 8 * BK);
-        } else {
-            const T* const row = reinterpret_cast<const T*>(j < kLoadsW ? w : x) + row_of(j) * (j < kLoadsW ? a.ldw : a.ldx);
-            staged[j] = load_vec<T, 8>(row + segment_of(j) * 8);
-        }
+        const unsigned offset = __umul24(row_of(j), (unsigned)(of_w(j) ? a.ldw : a.ldx) * 2) + segment_of(j) * 16;
+        dma_row(of_w(j) ? w : x, offset, lds + buffer * kRows * BK + piece(j) * 8 * BK);
     }
     __device__ __forceinline__ void read(int r, int buffer, int step, Frags& f) const
     {
@@ -225,62 +253,66 @@ struct Tile {
         }
     }
 
-    // Tile t, whose first fragments are in f0; leaves those of tile t + 1 there (behind the last tile: whatever the buffer holds).
-    template <bool LOAD>
-    __device__ __forceinline__ void tile(floatx4 (&acc)[FN][FM], Frags& f0, Frags& f1, int t, int k)
+    // Waits until at most `tiles` tiles (N at most) are on their way to LDS.
+    template <int N>
+    __device__ __forceinline__ static void wait_for_all_but_tiles(int tiles)
     {
-        const int b = t & 1;
+        if constexpr (N == 0) wait_for_all_but<0>();
+        else if (tiles >= N) wait_for_all_but<N * kLoads>();
+        else wait_for_all_but_tiles<N - 1>(tiles);
+    }
+
+    // The tile in buffer b, whose first fragments are in f0; leaves those of the next tile there (behind the last tile: whatever the buffer holds).
+    // With LOAD the tile that starts at column k takes its place.  `ahead` tiles may be on their way when the next one is needed.
+    template <bool LOAD>
+    __device__ __forceinline__ void tile(floatx4 (&acc)[FN][FM], Frags& f0, Frags& f1, int b, int ahead, int k)
+    {
+        const int next = b + 1 == S ? 0 : b + 1;
         step<false>(acc, f0, f1, b, 1, 0, nullptr, nullptr);
-        if constexpr (!DMA) {
-            if (t > 0) {
-#pragma unroll
-                for (int j = 0; j < kLoads; ++j) write(j, b ^ 1, staged[j]);
-            }
-        }
-        wait_all();
+        if constexpr (LOAD) wait_for_all_but<(S - 2) * kLoads>();
+        else wait_for_all_but_tiles<S - 2>(ahead);
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         const char *w = base_w + (int64_t)k * 2, *x = base_x + (int64_t)k * 2;
         asm volatile("" : "+s"(w), "+s"(x), "+v"(lane));        // (otherwise every piece's address is kept in registers and counted up)
-        step<LOAD>(acc, f1, f0, b ^ 1, 0, b, w, x);
+        step<LOAD>(acc, f1, f0, next, 0, b, w, x);
     }
 
     __device__ __forceinline__ void run(floatx4 (&acc)[FN][FM])
     {
-        const int whole = (int)(a.k / BK), ragged = a.k % BK ? 1 : 0, tiles = whole + ragged;
+        const int whole = columns / BK, ragged = columns % BK ? 1 : 0, tiles = whole + ragged;
         if (tiles == 0) return;
         // tile t starts at column first + t * 64, the ragged one (t = 0) at the end of the row
-        const int first = ragged ? -BK : 0;
+        const int first = ragged ? -BK : 0, filled = tiles < S ? tiles : S;
         __syncthreads();                                        // (the LDS of the tile before)
-        if (ragged) load_ragged(0, (int64_t)whole * BK);
-        else fill(0, 0);
-        if (tiles > 1) fill(1, first + BK);
-        wait_all();
-        __syncthreads();
+        for (int t = ragged; t < filled; ++t)
+#pragma unroll
+            for (int j = 0; j < kLoads; ++j) load(j, t, base_w + (int64_t)(first + t * BK) * 2, base_x + (int64_t)(first + t * BK) * 2);
+        if (ragged) load_ragged(0, whole * BK);
+        wait_for_all_but_tiles<S - 2>(ragged || filled < S ? 0 : S - 2);
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
         Frags f0, f1;
 #pragma unroll
         for (int r = 0; r < kReads; ++r) read(r, 0, 0, f0);
-        int t = 0;
-        for (; t + 2 < tiles; ++t) tile<true>(acc, f0, f1, t, first + (t + 2) * BK);
-        for (; t < tiles; ++t) tile<false>(acc, f0, f1, t, 0);
+        int t = 0, b = 0;
+        for (; t + S < tiles; ++t) {
+            tile<true>(acc, f0, f1, b, 0, first + (t + S) * BK);
+            b = b + 1 == S ? 0 : b + 1;
+        }
+        for (; t < tiles; ++t) {
+            tile<false>(acc, f0, f1, b, tiles - t - 2, 0);
+            b = b + 1 == S ? 0 : b + 1;
+        }
         if constexpr (kTied) settle();
     }
 
-    // a whole tile, at once (before the loop)
-    __device__ __forceinline__ void fill(int buffer, int k)
-    {
-#pragma unroll
-        for (int j = 0; j < kLoads; ++j) {
-            load(j, buffer, base_w + (int64_t)k * 2, base_x + (int64_t)k * 2);
-            if constexpr (!DMA) write(j, buffer, staged[j]);
-        }
-    }
-
     // The outputs pass through LDS, 16 rows of the wave's columns at a time, so that each row is written in whole lines.
-    __device__ __forceinline__ void store(const floatx4 (&acc)[FN][FM])
+    // `part`: where to put the bare sums ([m][n]) instead of finished outputs.
+    __device__ __forceinline__ void store(const floatx4 (&acc)[FN][FM], float* part)
     {
         constexpr int kColumns = FN * 16, kPitch = kColumns + 4;        // (16 bytes on: the rows of a fragment start in different banks)
-        static_assert(kWaves * 16 * kPitch * sizeof(float) <= 2 * kRows * BK * sizeof(T), "fits the tiles' LDS");
+        static_assert(kWaves * 16 * kPitch * sizeof(float) <= S * kRows * BK * sizeof(T), "fits the tiles' LDS");
         float* const mine = reinterpret_cast<float*>(lds) + wave * 16 * kPitch;
         __syncthreads();                                        // every wave has read its last fragments
 #pragma unroll 1
@@ -290,7 +322,7 @@ struct Tile {
                 if (q == j) {
 #pragma unroll
                     for (int i = 0; i < FN; ++i)
-                        *reinterpret_cast<floatx4*>(mine + (lane & 15) * kPitch + i * 16 + (lane >> 4) * 4) = acc[i][q] * a.alpha1;
+                        *reinterpret_cast<floatx4*>(mine + (lane & 15) * kPitch + i * 16 + (lane >> 4) * 4) = acc[i][q];
                 }
             __builtin_amdgcn_wave_barrier();
 #pragma unroll 1
@@ -303,7 +335,9 @@ struct Tile {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) v[h * 4 + r] = part[r];
                 }
-                finish<T>(a, m0 + ((wave / WN) * FM + j) * 16 + row, n0 + (wave % WN) * FN * 16 + column, v);
+                const int64_t m = m0 + ((wave / WN) * FM + j) * 16 + row, n = n0 + (wave % WN) * FN * 16 + column;
+                if (part) keep(a, part, m, n, v);
+                else finish<T>(a, m, n, v);
             }
             __builtin_amdgcn_wave_barrier();
         }
@@ -325,46 +359,259 @@ __device__ __forceinline__ void place(int64_t i, int64_t tiles_m, int64_t tiles_
     tn = in / height;
 }
 
-template <typename T, int FN, int FM, int WN, int WM, bool DMA>
-__global__ __launch_bounds__(WN * WM * 64, FN * FM > 32 ? 1 : 2)
-void dense_tile_kernel(dgnn_dense_args a, int64_t tiles_m, int64_t tiles_n)
+// `splits` shares of k, of `share` columns (a multiple of 64) each; with more than one, the sums go to `parts`.
+template <typename T, int FN, int FM, int WN, int WM, int S>
+__global__ __launch_bounds__(WN * WM * 64, (WN * WM * Tile<T, FN, FM, WN, WM, S>::kPerUnit + 3) / 4)
+void dense_tile_kernel(dgnn_dense_args a, int64_t tiles_m, int64_t tiles_n, int64_t splits, int64_t share, float* parts)
 {
-    typedef Tile<T, FN, FM, WN, WM, DMA> Work;
-    __shared__ __attribute__((aligned(1024))) T lds[2 * Work::kRows * Work::BK];
-    for (int64_t i = blockIdx.x; i < tiles_m * tiles_n; i += gridDim.x) {
+    typedef Tile<T, FN, FM, WN, WM, S> Work;
+    __shared__ __attribute__((aligned(1024))) T lds[S * Work::kRows * Work::BK];
+    const int64_t tiles = tiles_m * tiles_n;
+    for (int64_t i = blockIdx.x; i < tiles * splits; i += gridDim.x) {
+        const int64_t split = i / tiles, begin = split * share;
         int64_t tm, tn;
-        place(i, tiles_m, tiles_n, tm, tn);
-        Work work(a, lds, tm * Work::BM, tn * Work::BN);
+        place(i % tiles, tiles_m, tiles_n, tm, tn);
+        Work work(a, lds, tm * Work::BM, tn * Work::BN, begin, begin + share < a.k ? begin + share : a.k);
         floatx4 acc[FN][FM] = {};
         work.run(acc);
-        work.store(acc);
+        work.store(acc, parts ? parts + split * a.m * a.n : nullptr);
     }
 }
 
-template <typename T, int FN, int FM, int WN, int WM, bool DMA>
-hipError_t launch_tiles(const dgnn_dense_args& a, hipStream_t stream)
+// The shares' sums, in their order, and everything behind them.
+template <typename T>
+__global__ __launch_bounds__(256)
+void dense_join_kernel(dgnn_dense_args a, int64_t splits, const float* parts)
 {
-    typedef Tile<T, FN, FM, WN, WM, DMA> Work;
-    const int64_t tiles_m = (a.m + Work::BM - 1) / Work::BM, tiles_n = (a.n + Work::BN - 1) / Work::BN, tiles = tiles_m * tiles_n;
-    return launch(dense_tile_kernel<T, FN, FM, WN, WM, DMA>, dim3((unsigned)(tiles < kMaxGrid ? tiles : kMaxGrid)), dim3(Work::kThreads), stream, a, tiles_m, tiles_n);
+    const int64_t wide = (a.n + 7) / 8;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.m * wide; i += (int64_t)gridDim.x * 256) {
+        const int64_t m = i / wide, n = i % wide * 8;
+        float v[8] = {};
+        for (int64_t s = 0; s < splits; ++s) {
+            const float* const from = parts + (s * a.m + m) * a.n + n;
+            if (n + 8 <= a.n) {
+                const vec<float, 8> all = load_vec<float, 8>(from);
+#pragma unroll
+                for (int r = 0; r < 8; ++r) v[r] += all[r];
+            } else {
+#pragma unroll
+                for (int r = 0; r < 7; ++r)
+                    if (n + r < a.n) v[r] += from[r];
+            }
+        }
+        finish<T>(a, m, n, v);
+    }
 }
 
-bool sixteen(const void* p, int64_t stride, int64_t rows) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (rows <= 1 || stride % 8 == 0); }
+// Rows of any alignment -> rows that start at multiples of 16 bytes, zero behind their end.  Sixteen-bit types alone, so their bits.
+struct Packing {
+    const uint16_t* from;
+    uint16_t* to;
+    int64_t rows, ld;
+};
+__global__ __launch_bounds__(256)
+void dense_pack_kernel(Packing w, Packing x, int64_t k, int64_t pitch)
+{
+    const int64_t wide = pitch / 8;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (w.rows + x.rows) * wide; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i / wide, column = i % wide * 8;
+        const Packing& p = row < w.rows ? w : x;
+        const int64_t r = row < w.rows ? row : row - w.rows;
+        *reinterpret_cast<vec<uint16_t, 8>*>(p.to + r * pitch + column) = load_row<uint16_t>(p.from + r * p.ld, column, k);
+    }
+}
+
+// ---- few rows on one side: fragments straight from memory -------------------------------------------------------------------------
+//
+// Where one of the operands has few rows, or both are small, there is little to share through LDS: a workgroup owns 16 x 16 outputs, its waves
+// share the columns of k in contiguous pieces and fetch the fragments they multiply, and their sums meet in LDS, in order.  Rows need no alignment.
+// Bound by what a unit's L1 passes on: 28 GB/s a unit at 16 x 8192 x 512 (18 us on 32 units), 5.2 TB/s of HBM at 1 x 4096 x 16384 (25.8 us).
+constexpr int kDirectWaves = 16;
+template <typename T>
+__global__ __launch_bounds__(kDirectWaves * 64)
+void dense_direct_kernel(dgnn_dense_args a, int64_t tiles_n, int64_t tiles)
+{
+    constexpr int kPitch = 20, kUnroll = 8;
+    __shared__ __attribute__((aligned(16))) float partial[kDirectWaves][16][kPitch];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    const int steps = (int)((a.k + 31) / 32), whole = (int)(a.k / 32), each = (steps + waves - 1) / waves;
+    const int begin = wave * each, end = begin + each < steps ? begin + each : steps, full = end < whole ? end : whole;
+    for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+        const int64_t m0 = tile / tiles_n * 16, n0 = tile % tiles_n * 16;
+        // (beyond the last row: that one again, its outputs are not stored)
+        const int64_t n = n0 + (lane & 15), m = m0 + (lane & 15);
+        const T* const w = static_cast<const T*>(a.w) + (n < a.n ? n : a.n - 1) * a.ldw + (lane >> 4) * 8;
+        const T* const x = static_cast<const T*>(a.x) + (m < a.m ? m : a.m - 1) * a.ldx + (lane >> 4) * 8;
+        floatx4 acc = {};
+        int s = begin;
+        for (; s + kUnroll <= full; s += kUnroll) {
+            vec<T, 8> fw[kUnroll], fx[kUnroll];
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) {
+                fw[u] = load_vec<T, 8>(w + (int64_t)(s + u) * 32);
+                fx[u] = load_vec<T, 8>(x + (int64_t)(s + u) * 32);
+            }
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) acc = mfma<T>(fw[u], fx[u], acc);
+        }
+        for (; s < end; ++s) {
+            const int64_t left = a.k - (int64_t)s * 32 - (lane >> 4) * 8;
+            acc = mfma<T>(load_row<T>(w + (int64_t)s * 32, 0, left), load_row<T>(x + (int64_t)s * 32, 0, left), acc);
+        }
+        __syncthreads();                                                       // (the sums of the tile before)
+        *reinterpret_cast<floatx4*>(&partial[wave][lane & 15][(lane >> 4) * 4]) = acc;
+        __syncthreads();
+        for (int e = threadIdx.x; e < 32; e += blockDim.x) {
+            const int row = e >> 1, column = (e & 1) * 8;
+            float v[8] = {};
+            for (int g = 0; g < waves; ++g)
+#pragma unroll
+                for (int r = 0; r < 8; ++r) v[r] += partial[g][row][column + r];
+            finish<T>(a, m0 + row, n0 + column, v);
+        }
+    }
+}
+
+// ---- which form a call takes ---------------------------------------------------------------------------------------------------------
+//
+// A call is priced in every form it could take and takes the cheapest.  The prices are measured (microseconds, bf16): one tile of 64 columns
+// of k where a compute unit holds one workgroup, the same where it holds two, and what a workgroup takes besides (first loads, outputs).  What
+// a form costs beside its neighbours, at the sizes where they change places:
+//   16 x 4096 x 16384 (m, k, n)   direct 36.2   16 x 64: 24.9   32 x 32: 25.4
+//    1 x 2888 x 362               direct  6.4   32 x 32: 11.4
+//   64 x 4096 x 4096              32 x 32: 14.1   64 x 64: 22.5   64 x 128: 31.2
+//   64 x 4096 x 16384             32 x 32: 38.5   64 x 64: 28.4   64 x 128: 33.8
+//  512 x 4096 x 4096              64 x 64: 35.7   64 x 128: 31.5   128 x 128: 39.6   256 x 256: 98.9
+// 4096 x 4096 x 1024              64 x 128: 58.7   128 x 128: 41.4   256 x 256: 107
+// 4096 x 1024 x 4096              128 x 128: 53.4   256 x 256: 38.4
+struct Form {
+    int bm, bn, per_unit;
+    double alone, crowded, fixed;
+};
+constexpr Form kForms[] = {
+    {16, 64, 2, 0.27, 0.40, 2.5},
+    {64, 16, 2, 0.27, 0.40, 2.5},
+    {32, 32, 2, 0.19, 0.29, 2.2},
+    {64, 64, 2, 0.32, 0.48, 3.0},
+    {64, 128, 1, 0.47, 0.47, 3.3},
+    {128, 128, 1, 0.60, 0.60, 4.0},
+    {256, 256, 1, 1.72, 1.72, 12.0},
+};
+constexpr int kNumForms = sizeof(kForms) / sizeof(kForms[0]), kDirect = -1;
+constexpr double kUnits = 256;
+// One launch more: what it takes on the device and, where calls follow each other closely, the host.
+constexpr double kLaunch = 5.0;
+
+struct Plan {
+    int form = kDirect;
+    int64_t splits = 1, share = 0;          // shares of k, columns of each
+    bool pack_w = false, pack_x = false;    // rows are copied to where they can be fetched 16 bytes at a time
+    int64_t pitch = 0;                      // of packed rows
+    int64_t bytes_w = 0, bytes_x = 0, bytes_parts = 0;
+    int64_t workspace() const { return bytes_w + bytes_x + bytes_parts; }
+};
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
+
+// Rows the DMA can fetch: 16-byte aligned, and offsets inside a tile's 256 rows in 24 x 24 bits.
+bool fetchable(const void* p, int64_t stride, int64_t rows) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (rows <= 1 || (stride % 8 == 0 && stride < 1 << 22)); }
+
+Plan make_plan(const dgnn_dense_args& a)
+{
+    Plan best;
+    const int64_t tiles_k = ceil_div(a.k, 64);
+    const bool ready_w = fetchable(a.w, a.ldw, a.n), ready_x = fetchable(a.x, a.ldx, a.m);
+    // fragments straight from memory: bound by what a unit's L1 passes on; rows that are not there cost nothing, unaligned ones nearly twice
+    const double few = (double)(a.m < a.n ? a.m : a.n), tiles = (double)ceil_div(a.m, 16) * (double)ceil_div(a.n, 16);
+    double price = (tiles > kUnits ? tiles / kUnits : 1.0) * (double)tiles_k * (0.08 + 0.066 * (few < 16 ? few : 16) / 16) * (ready_w && ready_x ? 1.0 : 1.9) + 3.0;
+    if (a.k == 0) return best;
+    double packing = 0.0;
+    const int64_t pitch = round_up(a.k, 64);
+    if (!ready_w || !ready_x) {
+        if (pitch >= 1 << 22) return best;
+        packing = kLaunch + (double)((ready_w ? 0 : a.n) + (ready_x ? 0 : a.m)) * (double)pitch * 4 / 4.0e6;
+    }
+    for (int f = 0; f < kNumForms; ++f) {
+        const Form& form = kForms[f];
+        const double count = (double)ceil_div(a.m, form.bm) * (double)ceil_div(a.n, form.bn);
+        for (int64_t splits = 1; splits <= 16; ++splits) {
+            const int64_t share = round_up(ceil_div(a.k, splits), 64);
+            if (splits > 1 && (share < 256 || ceil_div(a.k, share) != splits || count * (double)splits > kUnits * form.per_unit)) continue;
+            const double all = count * (double)splits, slots = kUnits * (all <= kUnits ? 1 : form.per_unit);
+            const double rounds = (double)(int64_t)((all + slots - 1) / slots), each = (double)(share / 64) * (all <= kUnits ? form.alone : form.crowded) + form.fixed;
+            const double join = splits > 1 ? kLaunch + (double)splits * (double)a.m * (double)a.n * 8 / 3.0e6 : 0.0;
+            const double cost = rounds * each + join + packing;
+            if (cost >= price) continue;
+            price = cost;
+            best.form = f;
+            best.splits = splits;
+            best.share = share;
+        }
+    }
+    if (best.form == kDirect) return best;
+    best.pack_w = !ready_w;
+    best.pack_x = !ready_x;
+    best.pitch = pitch;
+    best.bytes_w = best.pack_w ? round_up(a.n * pitch * 2, 256) : 0;
+    best.bytes_x = best.pack_x ? round_up(a.m * pitch * 2, 256) : 0;
+    best.bytes_parts = best.splits > 1 ? best.splits * a.m * a.n * 4 : 0;
+    return best;
+}
+
+template <typename T, int FN, int FM, int WN, int WM, int S>
+hipError_t launch_tiles(const dgnn_dense_args& a, const Plan& plan, float* parts, hipStream_t stream)
+{
+    typedef Tile<T, FN, FM, WN, WM, S> Work;
+    const int64_t tiles_m = ceil_div(a.m, Work::BM), tiles_n = ceil_div(a.n, Work::BN), all = tiles_m * tiles_n * plan.splits;
+    return launch(dense_tile_kernel<T, FN, FM, WN, WM, S>, dim3((unsigned)(all < kMaxGrid ? all : kMaxGrid)), dim3(Work::kThreads), stream,
+                  a, tiles_m, tiles_n, plan.splits, plan.share, parts);
+}
 
 template <typename T>
-hipError_t launch_typed(const dgnn_dense_args& a, hipStream_t stream)
+hipError_t launch_direct(const dgnn_dense_args& a, hipStream_t stream)
 {
-    // an offset inside a tile's 256 rows is 32 bits
-    const bool dma = sixteen(a.x, a.ldx, a.m) && sixteen(a.w, a.ldw, a.n) && a.ldx < 1 << 22 && a.ldw < 1 << 22;
-    if (!dma) return launch_tiles<T, 4, 4, 2, 2, false>(a, stream);
-    const int64_t big = ((a.m + 255) / 256) * ((a.n + 255) / 256);
-    if (big >= 192) return launch_tiles<T, 4, 8, 4, 2, true>(a, stream);
-    const int64_t mid = ((a.m + 127) / 128) * ((a.n + 127) / 128);
-    if (mid >= 128) return launch_tiles<T, 4, 4, 2, 2, true>(a, stream);
-    return launch_tiles<T, 2, 2, 2, 2, true>(a, stream);
+    const int64_t tiles_n = ceil_div(a.n, 16), tiles = ceil_div(a.m, 16) * tiles_n, steps = ceil_div(a.k, 32);
+    int waves = 16;                                             // as many as give every unit sixteen, and each a few steps of its own
+    while (waves > 4 && (tiles * waves > 4096 || waves * 4 > steps)) waves /= 2;
+    return launch(dense_direct_kernel<T>, dim3((unsigned)(tiles < kMaxGrid ? tiles : kMaxGrid)), dim3(waves * 64), stream, a, tiles_n, tiles);
+}
+
+template <typename T>
+hipError_t launch_typed(dgnn_dense_args a, hipStream_t stream)
+{
+    const Plan plan = make_plan(a);
+    if (plan.form == kDirect) return launch_direct<T>(a, stream);
+    char* const memory = static_cast<char*>(a.workspace);
+    float* const parts = plan.splits > 1 ? reinterpret_cast<float*>(memory + plan.bytes_w + plan.bytes_x) : nullptr;
+    if (plan.pack_w || plan.pack_x) {
+        const Packing w{static_cast<const uint16_t*>(a.w), reinterpret_cast<uint16_t*>(memory), plan.pack_w ? a.n : 0, a.ldw};
+        const Packing x{static_cast<const uint16_t*>(a.x), reinterpret_cast<uint16_t*>(memory + plan.bytes_w), plan.pack_x ? a.m : 0, a.ldx};
+        const int64_t blocks = ceil_div((w.rows + x.rows) * (plan.pitch / 8), 256);
+        const hipError_t err = launch(dense_pack_kernel, dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), stream, w, x, a.k, plan.pitch);
+        if (err != hipSuccess) return err;
+        if (plan.pack_w) { a.w = w.to; a.ldw = plan.pitch; }
+        if (plan.pack_x) { a.x = x.to; a.ldx = plan.pitch; }
+        if (plan.pack_w && plan.pack_x) a.k = plan.pitch;       // the zeros behind the rows are as good as the rows' end
+    }
+    hipError_t err = hipErrorInvalidValue;
+    switch (plan.form) {
+    case 0: err = launch_tiles<T, 1, 1, 4, 1, 8>(a, plan, parts, stream); break;
+    case 1: err = launch_tiles<T, 1, 1, 1, 4, 8>(a, plan, parts, stream); break;
+    case 2: err = launch_tiles<T, 1, 1, 2, 2, 8>(a, plan, parts, stream); break;
+    case 3: err = launch_tiles<T, 2, 2, 2, 2, 4>(a, plan, parts, stream); break;
+    case 4: err = launch_tiles<T, 4, 2, 2, 2, 4>(a, plan, parts, stream); break;
+    case 5: err = launch_tiles<T, 4, 2, 2, 4, 4>(a, plan, parts, stream); break;
+    case 6: err = launch_tiles<T, 4, 8, 4, 2, 2>(a, plan, parts, stream); break;
+    }
+    if (err != hipSuccess || !parts) return err;
+    const int64_t blocks = ceil_div(a.m * ceil_div(a.n, 8), 256);
+    return launch(dense_join_kernel<T>, dim3((unsigned)(blocks < kMaxGrid ? blocks : kMaxGrid)), dim3(256), stream, a, plan.splits, parts);
 }
 
 }  // namespace
+
+int64_t dense_workspace(const dgnn_dense_args& a) { return make_plan(a).workspace(); }
 
 hipError_t launch_dense(const dgnn_dense_args& a, hipStream_t stream)
 {

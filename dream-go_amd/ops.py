@@ -26,6 +26,7 @@ OPS_LIB_PATH = os.environ.get("DGNN_OPS_LIBRARY") or os.path.join(os.path.dirnam
 # every symbol include/dgnn_ops.h declares: (name, restype, argtypes).  Argument blocks travel as packed bytes (the struct formats below).
 SYMBOLS = [
     ("dgnn_ops_last_hip_error", ctypes.c_int, []),
+    ("dgnn_dense_workspace", ctypes.c_int, [ctypes.c_char_p, ctypes.POINTER(ctypes.c_int64)]),
     ("dgnn_dense", ctypes.c_int, [ctypes.c_int, ctypes.c_void_p, ctypes.c_char_p]),
     ("dgnn_group_norm_workspace", ctypes.c_int, [ctypes.c_char_p, ctypes.POINTER(ctypes.c_int64)]),
     ("dgnn_group_norm", ctypes.c_int, [ctypes.c_int, ctypes.c_void_p, ctypes.c_char_p]),
@@ -37,7 +38,7 @@ _TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 _INTEGERS = {torch.int32: 3, torch.int64: 4}
 
 # dgnn_dense_args, dgnn_group_norm_args, dgnn_logits_args
-_DENSE = struct.Struct("@5P7q2f4i")
+_DENSE = struct.Struct("@6P8q2f4i")
 _GROUP_NORM = struct.Struct("@6P11qf3i")
 _LOGITS = struct.Struct("@10P8q3f4i4x")
 
@@ -178,8 +179,15 @@ def dense(x, weight, bias=None, residual=None, *, alpha1=1.0, alpha2=1.0, activa
         if out.shape != (*leading, n):
             _refuse(where, f"out is {tuple(out.shape)}, expected {(*leading, n)}")
         ldy = _rows(where, "out", _flat(where, "out", out, m), m, n)
-    block = _DENSE.pack(px, pw, pb, pz, py, m, n, k, ldx, ldw, ldz, ldy, alpha1, alpha2,
-                        _TYPES[dtype], _TYPES[out_dtype], bias_type, _activation(where, activation))
+    tail = (m, n, k, ldx, ldw, ldz, ldy, alpha1, alpha2, _TYPES[dtype], _TYPES[out_dtype], bias_type, _activation(where, activation))
+    block = _DENSE.pack(px, pw, pb, pz, py, 0, 0, *tail)
+    need = ctypes.c_int64()
+    status = lib.dgnn_dense_workspace(block, need)
+    if status:
+        _fail(status, where)
+    if need.value:
+        workspace = torch.empty(need.value, dtype=torch.uint8, device=device)
+        block = _DENSE.pack(px, pw, pb, pz, py, workspace.data_ptr(), need.value, *tail)
     status = lib.dgnn_dense(device.index, _stream(device), block)
     if status:
         _fail(status, where)

@@ -98,7 +98,9 @@ def dense_case(ops, m, n, k, dtype, out_dtype, activation, bias, residual, seed,
 SIZES = [(1, 1, 1), (1, 362, 2888), (1, 1, 722), (2, 3, 5), (3, 17, 31), (7, 64, 64), (15, 16, 33), (16, 48, 256), (17, 15, 8), (16, 1000, 520),
          (31, 33, 1031), (32, 96, 96), (33, 200, 40), (63, 65, 127), (64, 64, 64), (65, 129, 200), (100, 362, 722), (127, 255, 511), (128, 128, 128),
          (129, 130, 1000), (255, 257, 65), (256, 256, 512), (256, 362, 2888), (257, 300, 72), (300, 1, 722), (512, 512, 96), (600, 520, 1032),
-         (1000, 999, 333), (2049, 77, 24), (5000, 9, 9), (9, 5000, 9), (1, 9000, 40), (4, 4100, 2048), (1024, 1024, 1024), (769, 1025, 2056)]
+         (1000, 999, 333), (2049, 77, 24), (5000, 9, 9), (9, 5000, 9), (1, 9000, 40), (4, 4100, 2048), (1024, 1024, 1024), (769, 1025, 2056),
+         # shares of k, copies of unaligned rows, the largest tile with ragged edges, many rows on one side only
+         (16, 512, 8192), (8, 100, 20001), (33, 40, 16384), (700, 900, 1001), (2100, 1030, 515), (3500, 3700, 200), (3600, 3500, 263), (70000, 16, 72), (40, 30000, 80)]
 
 
 @pytest.mark.parametrize("m,n,k", SIZES)

@@ -37,7 +37,7 @@ def test_the_argument_blocks_are_the_headers_structs(ops, tmp_path):
         assert np.frombuffer(block.pack(*([0] * (len(block.unpack(bytes(block.size))) - 1)), 77), dtype=np.int32)[int(out[2 * i + 1]) // 4] == 77
 
 
-DENSE = dict(x=0x10000, w=0x20000, bias=0x30000, z=0x40000, y=0x50000, m=4, n=8, k=16, ldx=16, ldw=16, ldz=8, ldy=8, alpha1=1.0, alpha2=1.0,
+DENSE = dict(x=0x10000, w=0x20000, bias=0x30000, z=0x40000, y=0x50000, workspace=0x100000, workspace_bytes=1 << 40, m=4, n=8, k=16, ldx=16, ldw=16, ldz=8, ldy=8, alpha1=1.0, alpha2=1.0,
              type=F16, out_type=F16, bias_type=F16, activation=0)
 GROUP_NORM = dict(x=0x10000, weight=0x20000, bias=0x30000, z=0x40000, y=0x50000, workspace=0x100000, workspace_bytes=1 << 40, n=2, p=5, c=16,
                   groups=4, x_n=80, x_p=16, z_n=80, z_p=16, y_n=80, y_p=16, eps=1e-5, type=F16, affine_type=F32, activation=4)
@@ -111,6 +111,8 @@ def test_refusals(ops, base, changes, status):
 
 def test_null_argument_blocks(ops):
     need = ctypes.c_int64(5)
+    assert ops.lib.dgnn_dense_workspace(None, need) == BAD_ARGUMENT and need.value == 0
+    assert ops.lib.dgnn_dense_workspace(ops._DENSE.pack(*DENSE.values()), None) == BAD_ARGUMENT
     for fn in (ops.lib.dgnn_dense, ops.lib.dgnn_group_norm, ops.lib.dgnn_adjust_logits):
         assert fn(0, None, None) == BAD_ARGUMENT
     assert ops.lib.dgnn_group_norm_workspace(None, need) == BAD_ARGUMENT and need.value == 0
@@ -125,9 +127,23 @@ def test_a_workspace_that_is_too_small_is_refused(ops, shape):
     assert ops.lib.dgnn_group_norm_workspace(ops._GROUP_NORM.pack(*args.values()), need) == OK
     assert 0 <= need.value < 1 << 28
     if need.value:
-        for bad in (dict(workspace=0), dict(workspace_bytes=need.value - 1), dict(workspace=0x100008)):
+        for bad in (dict(workspace=0), dict(workspace_bytes=need.value - 1), dict(workspace=0x100080)):
             assert ops.lib.dgnn_group_norm(NO_DEVICE, None, ops._GROUP_NORM.pack(*{**args, **bad}.values())) == BAD_ARGUMENT
     assert ops.lib.dgnn_group_norm(NO_DEVICE, None, ops._GROUP_NORM.pack(*{**args, "workspace_bytes": need.value}.values())) == HIP_ERROR
+
+
+@pytest.mark.parametrize("m,n,k,first,pad", [(1, 362, 2888, 0, 0), (16, 512, 8192, 0, 0), (1000, 1000, 1001, 0, 0), (300, 300, 320, 2, 0), (4096, 4096, 4095, 0, 1),
+                                             (8192, 4096, 16384, 0, 0), (64, 64, 1 << 20, 0, 0), (1 << 20, 8, 64, 0, 0), (20, 20, (1 << 31) - 1, 0, 0)])
+def test_the_workspace_of_a_dense_layer(ops, m, n, k, first, pad):
+    args = dict(DENSE, x=(1 << 44) + first, w=1 << 45, y=1 << 46, z=0, m=m, n=n, k=k, ldx=k + pad, ldw=k, ldy=n)
+    need = ctypes.c_int64()
+    assert ops.lib.dgnn_dense_workspace(ops._DENSE.pack(*args.values()), need) == OK
+    # never more than a copy of both operands, rows rounded up, and sixteen times the outputs in fp32
+    assert 0 <= need.value <= 2 * (m + n) * (k + 64) + 64 * m * n + 512
+    if need.value:
+        for bad in (dict(workspace=0), dict(workspace_bytes=need.value - 1), dict(workspace=0x100080)):
+            assert ops.lib.dgnn_dense(NO_DEVICE, None, ops._DENSE.pack(*{**args, **bad}.values())) == BAD_ARGUMENT
+    assert ops.lib.dgnn_dense(NO_DEVICE, None, ops._DENSE.pack(*{**args, "workspace_bytes": need.value}.values())) == HIP_ERROR
 
 
 def test_tensors_of_the_cpu_are_refused(ops, api):
