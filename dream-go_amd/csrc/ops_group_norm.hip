@@ -40,10 +40,11 @@ struct Part {
     int channels;           // of the slab
     int row;                // of the workgroup's rows; -1: this thread has no part
     int at, c, n;           // first channel in the slab and of all, channels (fewer than a vector at the end of a slab)
+    int back;               // how far back a whole vector has to begin to end inside the row
 };
 
 template <int V>
-__device__ __forceinline__ Part part_of(const Layout& l, int groups, int slab)
+__device__ __forceinline__ Part part_of(const Layout& l, int channels, int groups, int slab)
 {
     Part p;
     const int row = threadIdx.x / l.lanes, lane = threadIdx.x - row * l.lanes;
@@ -67,18 +68,51 @@ __device__ __forceinline__ Part part_of(const Layout& l, int groups, int slab)
     p.n = p.channels - p.at < V ? p.channels - p.at : V;
     p.row = row < l.rows && p.n > 0 ? row : -1;
     if (p.row < 0) p.at = p.n = 0, p.c = c0;
+    p.back = p.c + V <= channels ? 0 : p.c + V - channels;
     return p;
 }
 
+// The vector `n` elements on: element e of what is returned is element e + n, n < V.
 template <typename T, int V>
-__device__ __forceinline__ vec<T, V> load_part(const T* p, int n)
+__device__ __forceinline__ vec<T, V> moved_down(vec<T, V> v, int n)
 {
-    if (n == V) return load_vec<T, V>(p);
-    vec<T, V> v = {};
+    typedef vec<unsigned, 4> Words;
+    Words w = __builtin_bit_cast(Words, v);
+    const unsigned bytes = n * sizeof(T) & 3;
+    if (n * (int)sizeof(T) & 8) w = Words{w[2], w[3], 0, 0};
+    if (n * (int)sizeof(T) & 4) w = Words{w[1], w[2], w[3], 0};
+    if (bytes) w = Words{__builtin_amdgcn_alignbyte(w[1], w[0], bytes), __builtin_amdgcn_alignbyte(w[2], w[1], bytes), __builtin_amdgcn_alignbyte(w[3], w[2], bytes), w[3] >> bytes * 8};
+    return __builtin_bit_cast(vec<T, V>, w);
+}
+
+// The thread's part of `here` rows (R at most), `step` elements apart; zeros behind a part's end and for the other rows.  All loads first, then
+// what makes them parts: the loads of a thread are on their way at once.  TINY: no row is as long as a vector.
+template <typename T, int R, int V, bool TINY>
+__device__ __forceinline__ void load_rows(const T* p, int64_t step, int here, const Part& part, vec<T, V> (&held)[R])
+{
+    if constexpr (TINY) {
 #pragma unroll
-    for (int e = 0; e < V; ++e)
-        if (e < n) v[e] = p[e];
-    return v;
+        for (int r = 0; r < R; ++r) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) held[r][e] = r < here && e < part.n ? p[e] : (T)0.0f;
+            p += step;
+        }
+        return;
+    }
+    p -= part.back;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        held[r] = r < here ? load_vec<T, V>(p) : vec<T, V>{};
+        p += step;
+    }
+    if (part.n < V) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            if (part.back > 0) held[r] = moved_down<T, V>(held[r], part.back);
+#pragma unroll
+            for (int e = 0; e < V; ++e) held[r][e] = e < part.n ? held[r][e] : (T)0.0f;
+        }
+    }
 }
 
 template <typename T, int V>
@@ -94,19 +128,25 @@ __device__ __forceinline__ void store_part(T* p, int n, const float (&v)[V])
 }
 
 template <typename T, int V>
-__device__ __forceinline__ void load_affine(const void* p, bool is_float, int c, int n, float otherwise, float (&v)[V])
+__device__ __forceinline__ void load_affine(const void* from, bool is_float, const Part& p, float otherwise, float (&v)[V])
 {
 #pragma unroll
     for (int e = 0; e < V; ++e) v[e] = otherwise;
-    if (!p) return;
-    if (is_float) {
+    if (!from || p.n <= 0) return;
+    if (p.back == 0) {                                          // (of the channels behind the part nothing is used)
+        if (is_float) {
+            const vec<float, V> all = load_vec<float, V>(static_cast<const float*>(from) + p.c);
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] = all[e];
+        } else {
+            const vec<T, V> all = load_vec<T, V>(static_cast<const T*>(from) + p.c);
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] = (float)all[e];
+        }
+    } else {
 #pragma unroll
         for (int e = 0; e < V; ++e)
-            if (e < n) v[e] = static_cast<const float*>(p)[c + e];
-    } else {
-        const vec<T, V> all = load_part<T, V>(static_cast<const T*>(p) + c, n);
-#pragma unroll
-        for (int e = 0; e < V; ++e) v[e] = (float)all[e];
+            if (e < p.n) v[e] = load_either<T>(from, p.c + e, is_float);
     }
 }
 
@@ -114,8 +154,8 @@ __device__ __forceinline__ void load_affine(const void* p, bool is_float, int c,
 template <int V>
 __device__ __forceinline__ void of_channels(const Layout& l, const Part& p, const float* of_group, float (&v)[V])
 {
-    if (l.subs > 1 || l.per % V == 0) {
-        const float all = of_group[l.subs > 1 ? 0 : p.at / l.per];
+    if (l.groups_per_slab == 1 || l.per % V == 0) {
+        const float all = of_group[l.groups_per_slab == 1 ? 0 : p.at / l.per];
 #pragma unroll
         for (int e = 0; e < V; ++e) v[e] = all;
     } else {
@@ -133,8 +173,8 @@ __device__ __forceinline__ void of_channels(const Layout& l, const Part& p, cons
 template <int V, typename Last>
 __device__ __forceinline__ void group_sums(const Layout& l, const Part& p, const float (&mine)[V], float* scratch, float* out, Last last)
 {
-    // a vector lies in one group, or (wide groups) the slab does: one number of each thread is enough
-    const bool single = l.subs > 1 || l.per % V == 0;
+    // a vector, or the whole slab, lies in one group: one number of each thread is enough
+    const bool single = l.groups_per_slab == 1 || l.per % V == 0;
     if (single) {
         float all = mine[0];
 #pragma unroll
@@ -146,8 +186,8 @@ __device__ __forceinline__ void group_sums(const Layout& l, const Part& p, const
     }
     __syncthreads();
     const int waves = (int)(blockDim.x + 63) >> 6, lane = threadIdx.x & 63;
-    const int pitch = single ? l.lanes : l.lanes * V, n = l.subs > 1 ? l.lanes : single ? l.per / V : l.per;
-    const int down = 64 / n, across = 64 - down * n;            // 64 numbers on
+    const int pitch = single ? l.lanes : l.lanes * V, n = l.groups_per_slab == 1 ? l.lanes : single ? l.per / V : l.per;
+    const int down = 64 / n, across = 64 - down * n;            // 64 numbers on (n is 512 at most: down may be 0)
     for (int g = threadIdx.x >> 6; g < p.groups; g += waves) {
         float sum = 0.0f;
         int row = lane / n, column = lane - row * n;
@@ -168,8 +208,8 @@ template <typename V>
 __device__ __forceinline__ void as_loaded(V& v) { asm volatile("" : "+v"(v)); }
 
 // R vectors per thread.
-template <typename T, int R, bool SKIP>
-__global__ __launch_bounds__(R == kRegisters ? kMaxThreads / 2 : kMaxThreads)
+template <typename T, int R, bool SKIP, bool TINY>
+__global__ __launch_bounds__(R == kRegisters ? kMaxThreads / 2 : kMaxThreads, 4)
 void one_pass_kernel(dgnn_group_norm_args a, Layout l)
 {
     constexpr int V = width_of<T>;
@@ -177,26 +217,15 @@ void one_pass_kernel(dgnn_group_norm_args a, Layout l)
     const float inverse = 1.0f / ((float)a.p * (float)l.per);
     for (int64_t i = blockIdx.z; i < a.n; i += gridDim.z)
         for (int slab = blockIdx.x; slab < l.slabs; slab += gridDim.x) {
-            const Part p = part_of<V>(l, (int)a.groups, slab);
+            const Part p = part_of<V>(l, (int)a.c, (int)a.groups, slab);
             const int here = p.row < 0 || p.row >= a.p ? 0 : (int)(a.p - 1 - p.row) / l.rows + 1;    // positions of this thread
-            const T* x = static_cast<const T*>(a.x) + i * a.x_n + p.row * a.x_p + p.c;
+            const T* const x = static_cast<const T*>(a.x) + i * a.x_n + p.row * a.x_p + p.c;
             vec<T, V> held[R], skip[SKIP ? R : 1];
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-                held[r] = r < here ? load_part<T, V>(x, p.n) : vec<T, V>{};
-                x += l.rows * a.x_p;
-            }
-            if constexpr (SKIP) {
-                const T* z = static_cast<const T*>(a.z) + i * a.z_n + p.row * a.z_p + p.c;
-#pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    skip[r] = r < here ? load_part<T, V>(z, p.n) : vec<T, V>{};
-                    z += l.rows * a.z_p;
-                }
-            }
+            load_rows<T, R, V, TINY>(x, l.rows * a.x_p, here, p, held);
+            if constexpr (SKIP) load_rows<T, R, V, TINY>(static_cast<const T*>(a.z) + i * a.z_n + p.row * a.z_p + p.c, l.rows * a.z_p, here, p, skip);
             float weight[V], bias[V], sum[V] = {}, mean[V], scale[V];
-            load_affine<T, V>(a.weight, a.affine_type == DGNN_F32, p.c, p.n, 1.0f, weight);
-            load_affine<T, V>(a.bias, a.affine_type == DGNN_F32, p.c, p.n, 0.0f, bias);
+            load_affine<T, V>(a.weight, a.affine_type == DGNN_F32, p, 1.0f, weight);
+            load_affine<T, V>(a.bias, a.affine_type == DGNN_F32, p, 0.0f, bias);
 #pragma unroll
             for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -248,41 +277,44 @@ struct Moments {
 
 // (mean, squares) of a share of the positions of a slab's groups, to moments[sample][group][share][sub].  Every thread joins what it reads as it
 // comes, channel by channel; the threads of a group are joined at the end.
-template <typename T>
-__global__ __launch_bounds__(kMaxThreads)
+template <typename T, bool TINY>
+__global__ __launch_bounds__(kMaxThreads / 2, 4)
 void moments_kernel(dgnn_group_norm_args a, Layout l, Moments* moments)
 {
     constexpr int V = width_of<T>, R = kRegisters;
-    __shared__ float scratch[2][kMaxThreads * V], means[kMaxGroups], squares[kMaxGroups];
+    __shared__ float scratch[2][kMaxThreads / 2 * V], means[kMaxGroups], squares[kMaxGroups];
     const int64_t begin = blockIdx.y * l.share, end = begin + l.share < a.p ? begin + l.share : a.p;
     for (int64_t i = blockIdx.z; i < a.n; i += gridDim.z)
         for (int slab = blockIdx.x; slab < l.slabs; slab += gridDim.x) {
-            const Part p = part_of<V>(l, (int)a.groups, slab);
+            const Part p = part_of<V>(l, (int)a.c, (int)a.groups, slab);
             const float inverse = 1.0f / ((float)(end - begin) * (float)(l.subs > 1 ? p.channels : l.per));
             float mean[V] = {}, square[V] = {}, count = 0.0f;
             if (p.row >= 0)
                 for (int64_t q = begin + p.row; q < end; q += R * l.rows) {
-                    const T* x = static_cast<const T*>(a.x) + i * a.x_n + q * a.x_p + p.c;
+                    const T* const x = static_cast<const T*>(a.x) + i * a.x_n + q * a.x_p + p.c;
                     const int here = end - q > (R - 1) * l.rows ? R : (int)(end - 1 - q) / l.rows + 1;
                     vec<T, V> held[R];
-#pragma unroll
-                    for (int r = 0; r < R; ++r) {
-                        held[r] = r < here ? load_part<T, V>(x, p.n) : vec<T, V>{};
-                        x += l.rows * a.x_p;
-                    }
+                    load_rows<T, R, V, TINY>(x, l.rows * a.x_p, here, p, held);
+                    float m[V];
                     const float each = 1.0f / (float)here, all = count + (float)here, part = (float)here / all, between = count * part;
 #pragma unroll
                     for (int e = 0; e < V; ++e) {
-                        float s = 0.0f, m2 = 0.0f;
+                        m[e] = 0.0f;
 #pragma unroll
-                        for (int r = 0; r < R; ++r) s += (float)held[r][e];
-                        const float m = s * each;
+                        for (int r = 0; r < R; ++r) m[e] += (float)held[r][e];
+                        m[e] *= each;
+                    }
+#pragma unroll
+                    for (int r = 0; r < R; ++r) as_loaded(held[r]);
+#pragma unroll
+                    for (int e = 0; e < V; ++e) {
+                        float m2 = 0.0f;
 #pragma unroll
                         for (int r = 0; r < R; ++r) {
-                            const float d = r < here ? (float)held[r][e] - m : 0.0f;
+                            const float d = r < here ? (float)held[r][e] - m[e] : 0.0f;
                             m2 = __builtin_fmaf(d, d, m2);
                         }
-                        const float d = m - mean[e];
+                        const float d = m[e] - mean[e];
                         mean[e] = __builtin_fmaf(d, part, mean[e]);
                         square[e] += __builtin_fmaf(d * d, between, m2);
                     }
@@ -305,8 +337,8 @@ void moments_kernel(dgnn_group_norm_args a, Layout l, Moments* moments)
         }
 }
 
-template <typename T, bool SKIP>
-__global__ __launch_bounds__(kMaxThreads)
+template <typename T, bool SKIP, bool TINY>
+__global__ __launch_bounds__(kMaxThreads / 2, 4)
 void apply_kernel(dgnn_group_norm_args a, Layout l, const Moments* moments)
 {
     constexpr int V = width_of<T>, R = kRegisters / 2;
@@ -316,7 +348,7 @@ void apply_kernel(dgnn_group_norm_args a, Layout l, const Moments* moments)
     const float inverse = 1.0f / ((float)a.p * (float)l.per);
     for (int64_t i = blockIdx.z; i < a.n; i += gridDim.z)
         for (int slab = blockIdx.x; slab < l.slabs; slab += gridDim.x) {
-            const Part p = part_of<V>(l, (int)a.groups, slab);
+            const Part p = part_of<V>(l, (int)a.c, (int)a.groups, slab);
             for (int g = threadIdx.x >> 6; g < p.groups; g += waves) {
                 const Moments* const of = moments + (i * a.groups + p.g0 + g) * pieces;
                 const auto count = [&](int piece) {
@@ -337,8 +369,8 @@ void apply_kernel(dgnn_group_norm_args a, Layout l, const Moments* moments)
             }
             __syncthreads();
             float weight[V], bias[V], mean[V], scale[V];
-            load_affine<T, V>(a.weight, a.affine_type == DGNN_F32, p.c, p.n, 1.0f, weight);
-            load_affine<T, V>(a.bias, a.affine_type == DGNN_F32, p.c, p.n, 0.0f, bias);
+            load_affine<T, V>(a.weight, a.affine_type == DGNN_F32, p, 1.0f, weight);
+            load_affine<T, V>(a.bias, a.affine_type == DGNN_F32, p, 0.0f, bias);
             of_channels<V>(l, p, means, mean);
             of_channels<V>(l, p, scales, scale);
 #pragma unroll
@@ -346,20 +378,12 @@ void apply_kernel(dgnn_group_norm_args a, Layout l, const Moments* moments)
             __syncthreads();                                    // (means and scales are the next slab's)
             if (p.row < 0) continue;
             for (int64_t q = begin + p.row; q < end; q += R * l.rows) {
-                const T* x = static_cast<const T*>(a.x) + i * a.x_n + q * a.x_p + p.c;
-                const T* z = SKIP ? static_cast<const T*>(a.z) + i * a.z_n + q * a.z_p + p.c : nullptr;
+                const T* const x = static_cast<const T*>(a.x) + i * a.x_n + q * a.x_p + p.c;
                 T* y = static_cast<T*>(a.y) + i * a.y_n + q * a.y_p + p.c;
                 const int here = end - q > (R - 1) * l.rows ? R : (int)(end - 1 - q) / l.rows + 1;
                 vec<T, V> held[R], skip[SKIP ? R : 1];
-#pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    held[r] = r < here ? load_part<T, V>(x, p.n) : vec<T, V>{};
-                    x += l.rows * a.x_p;
-                    if constexpr (SKIP) {
-                        skip[r] = r < here ? load_part<T, V>(z, p.n) : vec<T, V>{};
-                        z += l.rows * a.z_p;
-                    }
-                }
+                load_rows<T, R, V, TINY>(x, l.rows * a.x_p, here, p, held);
+                if constexpr (SKIP) load_rows<T, R, V, TINY>(static_cast<const T*>(a.z) + i * a.z_n + q * a.z_p + p.c, l.rows * a.z_p, here, p, skip);
 #pragma unroll
                 for (int r = 0; r < R; ++r)
                     if (r < here) {
@@ -393,67 +417,68 @@ int64_t groups_of_whole_lines(int64_t per, int64_t groups, int64_t vector)
 // One pass where a workgroup's registers hold a slab of a sample, two otherwise.
 Layout make_layout(const dgnn_group_norm_args& a, int* registers)
 {
+    constexpr int kThreads = kMaxThreads / 2;                   // (1024 of four vectors hold what 512 of eight do)
     const int vector = a.type == DGNN_F32 ? 4 : 8;
     Layout l;
     l.per = (int)(a.c / a.groups);
-    l.subs = (int)ceil_div(l.per, kMaxVectors * vector);
     l.shares = 1;
     l.share = a.p;
-    int64_t groups = l.subs > 1 ? 1 : groups_of_whole_lines(l.per, a.groups, vector);
-    const int64_t whole = groups;
-    const auto cut = [&]() {
+    int64_t groups;
+    const auto cut = [&](int64_t g, int subs) {
+        groups = g;
+        l.subs = subs;
         l.groups_per_slab = (int)groups;
-        l.slabs = (int)(l.subs > 1 ? a.groups * l.subs : ceil_div(a.groups, groups));
-        l.lanes = (int)(l.subs > 1 ? kMaxVectors : ceil_div(groups * l.per, vector));
+        l.slabs = (int)(subs > 1 ? a.groups * subs : ceil_div(a.groups, groups));
+        l.lanes = (int)(subs > 1 ? kMaxVectors : ceil_div(groups * l.per, vector));
     };
-    cut();
-    // rows that a workgroup holds: 512 threads of eight vectors each, or 1024 of four
-    const auto held = [&]() { return (int64_t)(kMaxThreads / 2 / l.lanes) * kRegisters; };
+    const auto held = [&]() { return (int64_t)(kThreads / l.lanes) * kRegisters; };
+    cut(groups_of_whole_lines(l.per, a.groups, vector), 1);
+    const int64_t whole = groups;
     *registers = 0;
-    if (l.subs == 1) {
-        // narrower slabs where these leave compute units idle, or do not fit and two vectors of a line would
-        while (groups > 1 && a.n * l.slabs < kUnitsWanted) groups = (groups + 1) / 2, cut();
-        while (groups > 1 && groups * l.per > 2 * vector && a.p > held()) groups = (groups + 1) / 2, cut();
-        if (a.p <= held()) {
-            // many vectors to a thread where there are enough workgroups for several on a unit, few where a call is one trip through the chip
-            const int wanted = a.n * l.slabs >= 2 * kUnitsWanted ? kRegisters : 2;
-            l.threads = 64;
-            while (l.threads < kMaxThreads / (wanted == kRegisters ? 2 : 1) && (l.threads < l.lanes || (int64_t)(l.threads / l.lanes) * wanted < a.p)) l.threads *= 2;
-            l.rows = l.threads / l.lanes;
-            const int64_t each = ceil_div(a.p, l.rows);
-            *registers = each <= 2 ? 2 : each <= 4 ? 4 : 8;
-            return l;
-        }
-        groups = whole;
-        cut();
+    // narrower slabs where these leave compute units idle, or do not fit and two vectors of a line would
+    while (groups > 1 && a.n * l.slabs < kUnitsWanted) cut((groups + 1) / 2, 1);
+    while (groups > 1 && groups * l.per > 2 * vector && a.p > held()) cut((groups + 1) / 2, 1);
+    if (a.p <= held()) {
+        // many vectors to a thread where there are enough workgroups for several on a unit, few where a call is one trip through the chip
+        const int wanted = a.n * l.slabs >= 2 * kUnitsWanted ? kRegisters : 2, most = wanted == kRegisters ? kThreads : kMaxThreads;
+        l.threads = 64;
+        while (l.threads < most && (l.threads < l.lanes || (int64_t)(l.threads / l.lanes) * wanted < a.p)) l.threads *= 2;
+        l.rows = l.threads / l.lanes;
+        const int64_t each = ceil_div(a.p, l.rows);
+        *registers = each <= 2 ? 2 : each <= 4 ? 4 : 8;
+        return l;
     }
-    l.threads = kMaxThreads;
+    const int subs = (int)ceil_div(l.per, kMaxVectors * vector);
+    cut(subs > 1 ? 1 : whole, subs);
+    l.threads = kThreads;
     l.rows = l.threads / l.lanes;
-    // shares enough for two workgroups on every unit, of whole trips through the registers
-    const int64_t trip = (int64_t)l.rows * kRegisters, trips = ceil_div(a.p, trip);
+    // shares enough for two workgroups on every unit
     int64_t shares = ceil_div(2 * kUnitsWanted, a.n * l.slabs);
-    shares = shares > kMaxShares ? kMaxShares : shares > trips ? trips : shares;
-    l.share = ceil_div(trips, shares) * trip;
+    if (shares > kMaxShares) shares = kMaxShares;
+    l.share = ceil_div(ceil_div(a.p, shares), l.rows) * l.rows;
     l.shares = (int)ceil_div(a.p, l.share);
     return l;
 }
 
-template <typename T>
+template <typename T, bool SKIP, bool TINY>
 hipError_t launch_typed(const dgnn_group_norm_args& a, hipStream_t stream)
 {
     int registers;
     const Layout l = make_layout(a, &registers);
     const dim3 grid((unsigned)(l.slabs < 65536 ? l.slabs : 65536), (unsigned)l.shares, (unsigned)(a.n < 32768 ? a.n : 32768)), block(l.threads);
-    switch (registers) {
-    case 2: return a.z ? launch(one_pass_kernel<T, 2, true>, grid, block, stream, a, l) : launch(one_pass_kernel<T, 2, false>, grid, block, stream, a, l);
-    case 4: return a.z ? launch(one_pass_kernel<T, 4, true>, grid, block, stream, a, l) : launch(one_pass_kernel<T, 4, false>, grid, block, stream, a, l);
-    case 8: return a.z ? launch(one_pass_kernel<T, 8, true>, grid, block, stream, a, l) : launch(one_pass_kernel<T, 8, false>, grid, block, stream, a, l);
-    }
+    if (registers == 2) return launch(one_pass_kernel<T, 2, SKIP, TINY>, grid, block, stream, a, l);
+    if (registers == 4) return launch(one_pass_kernel<T, 4, SKIP, TINY>, grid, block, stream, a, l);
+    if (registers == 8) return launch(one_pass_kernel<T, 8, SKIP, TINY>, grid, block, stream, a, l);
     Moments* const moments = static_cast<Moments*>(a.workspace);
-    const hipError_t err = launch(moments_kernel<T>, grid, block, stream, a, l, moments);
-    if (err != hipSuccess) return err;
-    const Moments* const done = moments;
-    return a.z ? launch(apply_kernel<T, true>, grid, block, stream, a, l, done) : launch(apply_kernel<T, false>, grid, block, stream, a, l, done);
+    const hipError_t err = launch(moments_kernel<T, TINY>, grid, block, stream, a, l, moments);
+    return err != hipSuccess ? err : launch(apply_kernel<T, SKIP, TINY>, grid, block, stream, a, l, static_cast<const Moments*>(moments));
+}
+
+template <typename T>
+hipError_t launch_type(const dgnn_group_norm_args& a, hipStream_t stream)
+{
+    if (a.c < width_of<T>) return a.z ? launch_typed<T, true, true>(a, stream) : launch_typed<T, false, true>(a, stream);
+    return a.z ? launch_typed<T, true, false>(a, stream) : launch_typed<T, false, false>(a, stream);
 }
 
 }  // namespace
@@ -468,9 +493,9 @@ int64_t group_norm_workspace(const dgnn_group_norm_args& a)
 hipError_t launch_group_norm(const dgnn_group_norm_args& a, hipStream_t stream)
 {
     switch (a.type) {
-    case DGNN_F16: return launch_typed<f16>(a, stream);
-    case DGNN_BF16: return launch_typed<bf16>(a, stream);
-    default: return launch_typed<float>(a, stream);
+    case DGNN_F16: return launch_type<f16>(a, stream);
+    case DGNN_BF16: return launch_type<bf16>(a, stream);
+    default: return launch_type<float>(a, stream);
     }
 }
 
