@@ -74,6 +74,9 @@ __device__ __forceinline__ float activate(float v, int activation)
     }
 }
 
+// Kinds of activation that a kernel may be made for: what it does not need would still have to be fetched with its instructions.
+enum Kind { kPlain, kSilu, kAny };              // identity and ReLU; SiLU; every one
+
 // One branch for several values.
 template <int N>
 __device__ __forceinline__ void activate(float (&v)[N], int activation)
@@ -98,18 +101,50 @@ __device__ __forceinline__ void activate(float (&v)[N], int activation)
     }
 }
 
+template <Kind K, int N>
+__device__ __forceinline__ void activate_kind(float (&v)[N], int activation)
+{
+    if constexpr (K == kAny) activate(v, activation);
+    else {
+#pragma unroll
+        for (int r = 0; r < N; ++r) v[r] = K == kSilu ? silu_of(v[r]) : activation == DGNN_ACT_RELU && v[r] < 0.0f ? 0.0f : v[r];
+    }
+}
+
+template <int Control>
+__device__ __forceinline__ float moved(float v)
+{
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), Control, 0xf, 0xf, true));
+}
+
 // The sum over a wave, the same in every lane.  Inside a row of sixteen lanes by data-parallel moves, which cost no trip through LDS.
 __device__ __forceinline__ float wave_sum(float v)
 {
-    const auto moved = [](float x, auto control) {
-        return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(control)::value, 0xf, 0xf, true));
-    };
-    v += moved(v, std::integral_constant<int, 0xb1>{});          // quad_perm [1, 0, 3, 2]
-    v += moved(v, std::integral_constant<int, 0x4e>{});          // quad_perm [2, 3, 0, 1]
-    v += moved(v, std::integral_constant<int, 0x141>{});         // row_half_mirror
-    v += moved(v, std::integral_constant<int, 0x140>{});         // row_mirror
+    v += moved<0xb1>(v);                // quad_perm [1, 0, 3, 2]
+    v += moved<0x4e>(v);                // quad_perm [2, 3, 0, 1]
+    v += moved<0x141>(v);               // row_half_mirror
+    v += moved<0x140>(v);               // row_mirror
     const auto row = [&](int lane) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane)); };
     return (row(0) + row(16)) + (row(32) + row(48));
+}
+
+// The sums over the lanes of a wave that are equal modulo `period` (a power of two up to 64, the same in the whole wave), in every
+// one of them -- in an order of its own: take one lane's.
+template <int N>
+__device__ __forceinline__ void periodic_sums(float (&v)[N], int period)
+{
+    const auto each = [&](auto sum) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] = sum(v[e]);
+    };
+    // both halves of a swap with itself: the lower partner's value in every lane, and the upper one's
+    const auto joined = [](auto both) { return __builtin_bit_cast(float, (unsigned)both[0]) + __builtin_bit_cast(float, (unsigned)both[1]); };
+    if (period <= 1) each([](float x) { return x + moved<0xb1>(x); });
+    if (period <= 2) each([](float x) { return x + moved<0x4e>(x); });
+    if (period <= 4) each([](float x) { return x + moved<0x124>(x); });          // row_ror 4: with the next one, the four lanes 4 apart
+    if (period <= 8) each([](float x) { return x + moved<0x128>(x); });          // row_ror 8
+    if (period <= 16) each([&](float x) { const unsigned b = __builtin_bit_cast(unsigned, x); return joined(__builtin_amdgcn_permlane16_swap(b, b, false, false)); });
+    if (period <= 32) each([&](float x) { const unsigned b = __builtin_bit_cast(unsigned, x); return joined(__builtin_amdgcn_permlane32_swap(b, b, false, false)); });
 }
 
 }  // namespace ops

@@ -171,31 +171,44 @@ __device__ __forceinline__ void of_channels(const Layout& l, const Part& p, cons
 // The sums of `mine` over the threads of each group of the slab, as `last` makes them, to out[group].  One barrier inside and one behind;
 // `scratch` is not the one of the call before.
 template <int V, typename Last>
-__device__ __forceinline__ void group_sums(const Layout& l, const Part& p, const float (&mine)[V], float* scratch, float* out, Last last)
+__device__ __forceinline__ void group_sums(const Layout& l, const Part& p, float (&mine)[V], float* scratch, float* out, Last last)
 {
     // a vector, or the whole slab, lies in one group: one number of each thread is enough
     const bool single = l.groups_per_slab == 1 || l.per % V == 0;
+    // rows of a power of two are added up within each wave first
+    const bool even = (l.lanes & (l.lanes - 1)) == 0 && l.lanes <= 64;
+    const int waves = (int)(blockDim.x + 63) >> 6, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int mine_at = even ? wave * l.lanes + lane : threadIdx.x;
     if (single) {
-        float all = mine[0];
+        float all[1] = {mine[0]};
 #pragma unroll
-        for (int e = 1; e < V; ++e) all += mine[e];
-        scratch[threadIdx.x] = all;
+        for (int e = 1; e < V; ++e) all[0] += mine[e];
+        if (even) periodic_sums(all, l.lanes);
+        if (!even || lane < l.lanes) scratch[mine_at] = all[0];
     } else {
+        if (even) periodic_sums(mine, l.lanes);
+        if (!even || lane < l.lanes) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) scratch[threadIdx.x * V + e] = mine[e];
+            for (int e = 0; e < V; ++e) scratch[mine_at * V + e] = mine[e];
+        }
     }
     __syncthreads();
-    const int waves = (int)(blockDim.x + 63) >> 6, lane = threadIdx.x & 63;
-    const int pitch = single ? l.lanes : l.lanes * V, n = l.groups_per_slab == 1 ? l.lanes : single ? l.per / V : l.per;
+    const int rows = even ? waves : l.rows, pitch = single ? l.lanes : l.lanes * V, n = l.groups_per_slab == 1 ? l.lanes : single ? l.per / V : l.per;
     const int down = 64 / n, across = 64 - down * n;            // 64 numbers on (n is 512 at most: down may be 0)
-    for (int g = threadIdx.x >> 6; g < p.groups; g += waves) {
+    for (int g = wave; g < p.groups; g += waves) {
+        const float* const of = scratch + g * n;
         float sum = 0.0f;
         int row = lane / n, column = lane - row * n;
-        while (row < l.rows) {
-            sum += scratch[row * pitch + g * n + column];
-            row += down;
-            column += across;
-            if (column >= n) column -= n, ++row;
+        while (row < rows) {
+            float four[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                four[q] = row < rows ? of[row * pitch + column] : 0.0f;
+                row += down;
+                column += across;
+                if (column >= n) column -= n, ++row;
+            }
+            sum += (four[0] + four[1]) + (four[2] + four[3]);
         }
         sum = wave_sum(sum);
         if (lane == 0) out[g] = last(sum);
@@ -208,7 +221,7 @@ template <typename V>
 __device__ __forceinline__ void as_loaded(V& v) { asm volatile("" : "+v"(v)); }
 
 // R vectors per thread.
-template <typename T, int R, bool SKIP, bool TINY>
+template <typename T, int R, Kind K, bool SKIP, bool TINY>
 __global__ __launch_bounds__(R == kRegisters ? kMaxThreads / 2 : kMaxThreads, 4)
 void one_pass_kernel(dgnn_group_norm_args a, Layout l)
 {
@@ -263,7 +276,7 @@ void one_pass_kernel(dgnn_group_norm_args a, Layout l)
                         v[e] = __builtin_fmaf((float)held[r][e] - mean[e], scale[e], bias[e]);
                         if constexpr (SKIP) v[e] += (float)skip[r][e];
                     }
-                    activate(v, a.activation);
+                    activate_kind<K>(v, a.activation);
                     store_part<T, V>(y, p.n, v);
                     y += l.rows * a.y_p;
                 }
@@ -275,8 +288,12 @@ struct Moments {
     float mean, squares;                                        // squares: sum of squared differences from the mean
 };
 
-// (mean, squares) of a share of the positions of a slab's groups, to moments[sample][group][share][sub].  Every thread joins what it reads as it
-// comes, channel by channel; the threads of a group are joined at the end.
+// (mean, squares) of a share of the positions of a slab's groups, to moments[sample][group][share][sub].
+//
+// Each thread sums, channel by channel, the differences of its rows from its FIRST row and their squares: four operations a value, where a second
+// look at the values would take six, and this kernel is bound by them as much as by memory.  The shift is one of the n values it is taken from, so
+// n (mean - shift)^2 is less than n times the sum of squares about the mean, whatever the values are: n times a rounding is all that the
+// difference `square - sum^2 / n` can lose.  The threads of a group are then joined about their common mean.
 template <typename T, bool TINY>
 __global__ __launch_bounds__(kMaxThreads / 2, 4)
 void moments_kernel(dgnn_group_norm_args a, Layout l, Moments* moments)
@@ -288,41 +305,54 @@ void moments_kernel(dgnn_group_norm_args a, Layout l, Moments* moments)
         for (int slab = blockIdx.x; slab < l.slabs; slab += gridDim.x) {
             const Part p = part_of<V>(l, (int)a.c, (int)a.groups, slab);
             const float inverse = 1.0f / ((float)(end - begin) * (float)(l.subs > 1 ? p.channels : l.per));
-            float mean[V] = {}, square[V] = {}, count = 0.0f;
-            if (p.row >= 0)
-                for (int64_t q = begin + p.row; q < end; q += R * l.rows) {
-                    const T* const x = static_cast<const T*>(a.x) + i * a.x_n + q * a.x_p + p.c;
-                    const int here = end - q > (R - 1) * l.rows ? R : (int)(end - 1 - q) / l.rows + 1;
+            const int rows = (int)(end - begin), here = p.row < 0 || p.row >= rows ? 0 : (rows - 1 - p.row) / l.rows + 1;
+            float shift[V] = {}, sum[V] = {}, square[V] = {};
+            if (here > 0) {
+                const int64_t step = l.rows * a.x_p;
+                const T* x = static_cast<const T*>(a.x) + i * a.x_n + (begin + p.row) * a.x_p + p.c;
+                vec<T, V> first[1];
+                load_rows<T, 1, V, TINY>(x, step, 1, p, first);
+#pragma unroll
+                for (int e = 0; e < V; ++e) shift[e] = (float)first[0][e];
+                int done = 0;
+                for (; done + R <= here; done += R) {
                     vec<T, V> held[R];
-                    load_rows<T, R, V, TINY>(x, l.rows * a.x_p, here, p, held);
-                    float m[V];
-                    const float each = 1.0f / (float)here, all = count + (float)here, part = (float)here / all, between = count * part;
+                    load_rows<T, R, V, TINY>(x, step, R, p, held);
+                    x += R * step;
 #pragma unroll
-                    for (int e = 0; e < V; ++e) {
-                        m[e] = 0.0f;
+                    for (int r = 0; r < R; ++r)
 #pragma unroll
-                        for (int r = 0; r < R; ++r) m[e] += (float)held[r][e];
-                        m[e] *= each;
-                    }
-#pragma unroll
-                    for (int r = 0; r < R; ++r) as_loaded(held[r]);
-#pragma unroll
-                    for (int e = 0; e < V; ++e) {
-                        float m2 = 0.0f;
-#pragma unroll
-                        for (int r = 0; r < R; ++r) {
-                            const float d = r < here ? (float)held[r][e] - m[e] : 0.0f;
-                            m2 = __builtin_fmaf(d, d, m2);
+                        for (int e = 0; e < V; ++e) {
+                            const float d = (float)held[r][e] - shift[e];
+                            sum[e] += d;
+                            square[e] = __builtin_fmaf(d, d, square[e]);
                         }
-                        const float d = m[e] - mean[e];
-                        mean[e] = __builtin_fmaf(d, part, mean[e]);
-                        square[e] += __builtin_fmaf(d * d, between, m2);
-                    }
-                    count = all;
                 }
-            float mine[V], joint[V];
+                if (done < here) {
+                    vec<T, V> held[R];
+                    load_rows<T, R, V, TINY>(x, step, here - done, p, held);
 #pragma unroll
-            for (int e = 0; e < V; ++e) mine[e] = e < p.n ? mean[e] * count : 0.0f;
+                    for (int r = 0; r < R; ++r)
+                        if (done + r < here) {
+#pragma unroll
+                            for (int e = 0; e < V; ++e) {
+                                const float d = (float)held[r][e] - shift[e];
+                                sum[e] += d;
+                                square[e] = __builtin_fmaf(d, d, square[e]);
+                            }
+                        }
+                }
+            }
+            const float count = (float)here, each = here > 0 ? 1.0f / count : 0.0f;
+            float mean[V], mine[V], joint[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float about = sum[e] * each;
+                square[e] = __builtin_fmaf(-about, sum[e], square[e]);
+                square[e] = square[e] < 0.0f ? 0.0f : square[e];       // (a NaN stays)
+                mean[e] = shift[e] + about;
+                mine[e] = e < p.n ? mean[e] * count : 0.0f;
+            }
             group_sums<V>(l, p, mine, scratch[0], means, [&](float s) { return s * inverse; });
             of_channels<V>(l, p, means, joint);
 #pragma unroll
@@ -337,7 +367,7 @@ void moments_kernel(dgnn_group_norm_args a, Layout l, Moments* moments)
         }
 }
 
-template <typename T, bool SKIP, bool TINY>
+template <typename T, Kind K, bool SKIP, bool TINY>
 __global__ __launch_bounds__(kMaxThreads / 2, 4)
 void apply_kernel(dgnn_group_norm_args a, Layout l, const Moments* moments)
 {
@@ -357,12 +387,30 @@ void apply_kernel(dgnn_group_norm_args a, Layout l, const Moments* moments)
                     const int wide = l.subs == 1 || l.per - from < kMaxVectors * V ? l.per - from : kMaxVectors * V;
                     return (float)(left < l.share ? left : l.share) * (float)wide;
                 };
-                float sum = 0.0f, squares = 0.0f;
-                for (int piece = threadIdx.x & 63; piece < pieces; piece += 64) sum = __builtin_fmaf(of[piece].mean, count(piece), sum);
+                // four of a lane's pieces at a time, asked for together; up to 256 pieces are still there for the second sum
+                Moments m[4];
+                float c[4], sum = 0.0f, squares = 0.0f;
+                const auto fetch = [&](int base) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int piece = base + q * 64 + (threadIdx.x & 63);
+                        m[q] = piece < pieces ? of[piece] : Moments{0.0f, 0.0f};
+                        c[q] = piece < pieces ? count(piece) : 0.0f;
+                    }
+                };
+                for (int base = 0; base < pieces; base += 256) {
+                    fetch(base);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) sum = __builtin_fmaf(m[q].mean, c[q], sum);
+                }
                 const float mean = wave_sum(sum) * inverse;
-                for (int piece = threadIdx.x & 63; piece < pieces; piece += 64) {
-                    const float d = of[piece].mean - mean;
-                    squares += __builtin_fmaf(d * d, count(piece), of[piece].squares);
+                for (int base = 0; base < pieces; base += 256) {
+                    if (pieces > 256) fetch(base);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const float d = m[q].mean - mean;
+                        squares += __builtin_fmaf(d * d, c[q], m[q].squares);
+                    }
                 }
                 squares = wave_sum(squares);
                 if ((threadIdx.x & 63) == 0) means[g] = mean, scales[g] = 1.0f / sqrtf(__builtin_fmaf(squares, inverse, a.eps));
@@ -393,7 +441,7 @@ void apply_kernel(dgnn_group_norm_args a, Layout l, const Moments* moments)
                             v[e] = __builtin_fmaf((float)held[r][e] - mean[e], scale[e], bias[e]);
                             if constexpr (SKIP) v[e] += (float)skip[r][e];
                         }
-                        activate(v, a.activation);
+                        activate_kind<K>(v, a.activation);
                         store_part<T, V>(y, p.n, v);
                         y += l.rows * a.y_p;
                     }
@@ -439,8 +487,9 @@ Layout make_layout(const dgnn_group_norm_args& a, int* registers)
     while (groups > 1 && a.n * l.slabs < kUnitsWanted) cut((groups + 1) / 2, 1);
     while (groups > 1 && groups * l.per > 2 * vector && a.p > held()) cut((groups + 1) / 2, 1);
     if (a.p <= held()) {
-        // many vectors to a thread where there are enough workgroups for several on a unit, few where a call is one trip through the chip
-        const int wanted = a.n * l.slabs >= 2 * kUnitsWanted ? kRegisters : 2, most = wanted == kRegisters ? kThreads : kMaxThreads;
+        // as many vectors to a thread as give every unit 1024 of them: few where a call is one trip through the chip
+        const int64_t each_unit = a.n * l.slabs * l.lanes * a.p / (kUnitsWanted * kMaxThreads);
+        const int wanted = each_unit >= 6 ? kRegisters : each_unit >= 3 ? 4 : 2, most = wanted == kRegisters ? kThreads : kMaxThreads;
         l.threads = 64;
         while (l.threads < most && (l.threads < l.lanes || (int64_t)(l.threads / l.lanes) * wanted < a.p)) l.threads *= 2;
         l.rows = l.threads / l.lanes;
@@ -460,25 +509,33 @@ Layout make_layout(const dgnn_group_norm_args& a, int* registers)
     return l;
 }
 
-template <typename T, bool SKIP, bool TINY>
-hipError_t launch_typed(const dgnn_group_norm_args& a, hipStream_t stream)
+template <typename T, Kind K, bool SKIP, bool TINY>
+hipError_t launch_kind(const dgnn_group_norm_args& a, hipStream_t stream)
 {
     int registers;
     const Layout l = make_layout(a, &registers);
     const dim3 grid((unsigned)(l.slabs < 65536 ? l.slabs : 65536), (unsigned)l.shares, (unsigned)(a.n < 32768 ? a.n : 32768)), block(l.threads);
-    if (registers == 2) return launch(one_pass_kernel<T, 2, SKIP, TINY>, grid, block, stream, a, l);
-    if (registers == 4) return launch(one_pass_kernel<T, 4, SKIP, TINY>, grid, block, stream, a, l);
-    if (registers == 8) return launch(one_pass_kernel<T, 8, SKIP, TINY>, grid, block, stream, a, l);
+    if (registers == 2) return launch(one_pass_kernel<T, 2, K, SKIP, TINY>, grid, block, stream, a, l);
+    if (registers == 4) return launch(one_pass_kernel<T, 4, K, SKIP, TINY>, grid, block, stream, a, l);
+    if (registers == 8) return launch(one_pass_kernel<T, 8, K, SKIP, TINY>, grid, block, stream, a, l);
     Moments* const moments = static_cast<Moments*>(a.workspace);
     const hipError_t err = launch(moments_kernel<T, TINY>, grid, block, stream, a, l, moments);
-    return err != hipSuccess ? err : launch(apply_kernel<T, SKIP, TINY>, grid, block, stream, a, l, static_cast<const Moments*>(moments));
+    return err != hipSuccess ? err : launch(apply_kernel<T, K, SKIP, TINY>, grid, block, stream, a, l, static_cast<const Moments*>(moments));
+}
+
+template <typename T, bool SKIP>
+hipError_t launch_skip(const dgnn_group_norm_args& a, hipStream_t stream)
+{
+    if (a.c < width_of<T>) return launch_kind<T, kAny, SKIP, true>(a, stream);
+    if (a.activation == DGNN_ACT_IDENTITY || a.activation == DGNN_ACT_RELU) return launch_kind<T, kPlain, SKIP, false>(a, stream);
+    if (a.activation == DGNN_ACT_SILU) return launch_kind<T, kSilu, SKIP, false>(a, stream);
+    return launch_kind<T, kAny, SKIP, false>(a, stream);
 }
 
 template <typename T>
 hipError_t launch_type(const dgnn_group_norm_args& a, hipStream_t stream)
 {
-    if (a.c < width_of<T>) return a.z ? launch_typed<T, true, true>(a, stream) : launch_typed<T, false, true>(a, stream);
-    return a.z ? launch_typed<T, true, false>(a, stream) : launch_typed<T, false, false>(a, stream);
+    return a.z ? launch_skip<T, true>(a, stream) : launch_skip<T, false>(a, stream);
 }
 
 }  // namespace
