@@ -9,16 +9,22 @@ namespace dgnn {
 namespace ops {
 
 // Launches `kernel` and returns what the launch itself said (hipGetLastError would also return, and clear, what others left there).
+// `shared`: bytes of LDS beyond what the kernel declares, 64 KiB at most.
 template <typename... Params>
-hipError_t launch_as(void (*kernel)(Params...), dim3 grid, dim3 block, hipStream_t stream, Params... args)
+hipError_t launch_as(void (*kernel)(Params...), dim3 grid, dim3 block, size_t shared, hipStream_t stream, Params... args)
 {
     void* pointers[] = {const_cast<void*>(static_cast<const void*>(&args))...};
-    return hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, block, pointers, 0, stream);
+    return hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, block, pointers, shared, stream);
+}
+template <typename... Params, typename... Args>
+hipError_t launch_shared(void (*kernel)(Params...), dim3 grid, dim3 block, size_t shared, hipStream_t stream, Args... args)
+{
+    return launch_as<Params...>(kernel, grid, block, shared, stream, args...);
 }
 template <typename... Params, typename... Args>
 hipError_t launch(void (*kernel)(Params...), dim3 grid, dim3 block, hipStream_t stream, Args... args)
 {
-    return launch_as<Params...>(kernel, grid, block, stream, args...);
+    return launch_as<Params...>(kernel, grid, block, 0, stream, args...);
 }
 
 // A grid dimension times the workgroup's has to stay below 2^32; kernels loop over what a capped grid leaves.
