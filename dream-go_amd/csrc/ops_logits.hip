@@ -1,7 +1,7 @@
 // dgnn_adjust_logits: penalties for repeated tokens, biases and masks, one pass over the logits.
 //
-// A workgroup owns a chunk of one row's vocabulary.  Its logits, bias and mask are asked for first; while they are on their way it counts the
-// row's history into LDS -- the tokens of its chunk only, by integer atomics, whose order does not show -- and then adjusts and writes what it
+// A workgroup owns a chunk of one row's vocabulary.  Its logits and mask are asked for first; while they are on their way it counts the row's
+// history into LDS -- the tokens of its chunk only, by integer atomics, whose order does not show -- and then adjusts and writes what it
 // has.  Memory bounds it as long as a history is short beside the vocabulary: every chunk reads the whole history (out of the L2), so chunks are as
 // large as LDS allows two of on a compute unit, and smaller only where that leaves units idle.
 #include "ops_device.h"
@@ -12,7 +12,12 @@ namespace {
 
 constexpr int kMaxChunk = 16384, kMinChunk = 1024;      // tokens; 4 bytes of LDS each
 constexpr int kEach = 2;                                // vectors of eight tokens that a thread holds at a time
-constexpr unsigned kPrompt = 0x80000000u;               // the token occurs in the given part; the bits below count the answer part
+
+// What is counted of a token: how often it occurs in the given part, above, and in the answer part, below.  A history of fewer than 65536 tokens
+// fits sixteen bits each, and one kind of atomic does; with LONG one bit says that the given part has it at all.
+constexpr unsigned kLongHistory = 65536;
+template <bool LONG> constexpr unsigned kPrompt = LONG ? 0x80000000u : 0x10000u;
+template <bool LONG> constexpr unsigned kAnswers = kPrompt<LONG> - 1;
 
 template <typename T>
 __device__ __forceinline__ vec<float, 8> load_eight(const T* p)
@@ -21,8 +26,8 @@ __device__ __forceinline__ vec<float, 8> load_eight(const T* p)
 }
 
 // HISTORY: H is the type of its tokens.
-template <typename T, typename O, typename H, bool HISTORY>
-__global__ __launch_bounds__(1024)
+template <typename T, typename O, typename H, bool HISTORY, bool LONG>
+__global__ __launch_bounds__(1024, 8)                   // two workgroups on a unit: one counts while the other writes
 void logits_kernel(dgnn_logits_args a, int chunk, int chunks)
 {
     extern __shared__ __attribute__((aligned(16))) unsigned seen[];             // [chunk] with HISTORY
@@ -36,18 +41,15 @@ void logits_kernel(dgnn_logits_args a, int chunk, int chunks)
             const char* const bias = a.bias ? static_cast<const char*>(a.bias) + (i * a.ld_bias + v0) * (bias_is_float ? 4 : (int)sizeof(T)) : nullptr;
             O* const out = static_cast<O*>(a.out) + i * a.ld_out + v0;
             vec<T, 8> held[kEach];
-            vec<float, 8> shift[kEach];
             unsigned allowed[kEach];
             const auto fetch = [&](int base) {
 #pragma unroll
                 for (int q = 0; q < kEach; ++q) {
                     const int e = base + (q * (int)blockDim.x + (int)threadIdx.x) * 8;
                     held[q] = vec<T, 8>{};
-                    shift[q] = vec<float, 8>{};
                     allowed[q] = 0xff;
                     if (e + 8 <= n) {
                         held[q] = load_vec<T, 8>(logits + e);
-                        if (bias) shift[q] = bias_is_float ? load_eight(reinterpret_cast<const float*>(bias) + e) : load_eight(reinterpret_cast<const T*>(bias) + e);
                         if (mask) allowed[q] = mask[e >> 3];
                     }
                 }
@@ -68,10 +70,12 @@ void logits_kernel(dgnn_logits_args a, int chunk, int chunks)
                 __syncthreads();
                 const H* const history = static_cast<const H*>(a.history) + i * a.ld_history;
                 const auto note = [&](H token, int e) {
-                    const int64_t at = (int64_t)token - v0;
-                    if ((uint64_t)at < (uint64_t)n) {
-                        if (e < prompt) atomicOr(&seen[at], kPrompt);
-                        else atomicAdd(&seen[at], 1u);
+                    const auto at = (std::make_unsigned_t<H>)(token - (H)v0);      // (v0 < 2^31; a token below it becomes a large number)
+                    if (LONG && e < prompt) {
+                        if (at < (std::make_unsigned_t<H>)n) atomicOr(&seen[at], kPrompt<LONG>);
+                    } else {
+                        const unsigned one = e < prompt ? kPrompt<LONG> : 1u;
+                        if (at < (std::make_unsigned_t<H>)n) atomicAdd(&seen[at], one);
                     }
                 };
                 const int whole = length & ~3;
@@ -83,15 +87,10 @@ void logits_kernel(dgnn_logits_args a, int chunk, int chunks)
                 if (whole + (int)threadIdx.x < length) note(history[whole + threadIdx.x], whole + threadIdx.x);
                 __syncthreads();
             }
-            // l, with `count` as the history left it
-            const auto adjust = [&](float l, unsigned count, float add, bool keep) {
-                if constexpr (HISTORY) {
-                    const unsigned answered = count & ~kPrompt;
-                    const float p = l * (l > 0.0f ? inverse : repetition);
-                    l = count ? p : l;
-                    l = l - frequency * (float)answered - (answered ? presence : 0.0f);
-                }
-                return keep ? l + add : -INFINITY;
+            const auto penalize = [&](float l, unsigned count) {
+                const unsigned answered = count & kAnswers<LONG>;
+                const float p = l * (l > 0.0f ? inverse : repetition) - frequency * (float)answered;
+                return count ? p - (answered ? presence : 0.0f) : l;
             };
             for (int base = 0; base < n; base += kEach * 8 * blockDim.x) {
                 if (base > 0) fetch(base);
@@ -99,21 +98,28 @@ void logits_kernel(dgnn_logits_args a, int chunk, int chunks)
                 for (int q = 0; q < kEach; ++q) {
                     const int e = base + (q * (int)blockDim.x + (int)threadIdx.x) * 8;
                     if (e + 8 <= n) {
-                        vec<unsigned, 4> counts[2] = {};
+                        vec<float, 8> l = __builtin_convertvector(held[q], vec<float, 8>);
                         if constexpr (HISTORY) {
-                            counts[0] = *reinterpret_cast<const vec<unsigned, 4>*>(seen + e);
-                            counts[1] = *reinterpret_cast<const vec<unsigned, 4>*>(seen + e + 4);
-                        }
-                        vec<O, 8> to;
+                            const vec<unsigned, 8> counts = *reinterpret_cast<const vec<unsigned, 8>*>(seen + e);
 #pragma unroll
-                        for (int r = 0; r < 8; ++r) to[r] = (O)adjust((float)held[q][r], counts[r >> 2][r & 3], shift[q][r], allowed[q] >> r & 1);
-                        store_vec<O, 8>(out + e, to);
+                            for (int r = 0; r < 8; ++r)
+                                if (__builtin_amdgcn_ballot_w64(counts[r] != 0)) l[r] = penalize(l[r], counts[r]);      // (most of a vocabulary is never seen)
+                        }
+                        if (bias) l += bias_is_float ? load_eight(reinterpret_cast<const float*>(bias) + e) : load_eight(reinterpret_cast<const T*>(bias) + e);
+                        if (mask) {
+#pragma unroll
+                            for (int r = 0; r < 8; ++r) l[r] = allowed[q] & 1u << r ? l[r] : -INFINITY;
+                        }
+                        store_vec<O, 8>(out + e, __builtin_convertvector(l, vec<O, 8>));
                     } else {
                         for (int r = e; r < n; ++r) {
-                            const float add = bias ? load_either<T>(bias, r, bias_is_float) : 0.0f;
-                            out[r] = (O)adjust((float)logits[r], HISTORY ? seen[r] : 0u, add, !mask || (mask[r >> 3] >> (r & 7) & 1));
+                            float l = (float)logits[r];
+                            if constexpr (HISTORY) l = penalize(l, seen[r]);
+                            if (bias) l += load_either<T>(bias, r, bias_is_float);
+                            out[r] = (O)(!mask || (mask[r >> 3] >> (r & 7) & 1) ? l : -INFINITY);
                         }
                     }
+                    __builtin_amdgcn_sched_barrier(0);          // (one vector after the other: together they take more registers than there are)
                 }
             }
         }
@@ -137,10 +143,13 @@ hipError_t launch_typed(const dgnn_logits_args& a, hipStream_t stream)
     threads = threads < 64 ? 64 : threads > 1024 ? 1024 : threads;
     const int chunks = (int)((a.v + chunk - 1) / chunk);
     const dim3 grid((unsigned)(chunks < (1 << 20) ? chunks : 1 << 20), (unsigned)(a.b < 65535 ? a.b : 65535));
-    if (!history) return launch(logits_kernel<T, O, int32_t, false>, grid, dim3(threads), stream, a, chunk, chunks);
+    if (!history) return launch(logits_kernel<T, O, int32_t, false, false>, grid, dim3(threads), stream, a, chunk, chunks);
     const size_t shared = chunk * sizeof(unsigned);
-    if (a.history_type == DGNN_I64) return launch_shared(logits_kernel<T, O, int64_t, true>, grid, dim3(threads), shared, stream, a, chunk, chunks);
-    return launch_shared(logits_kernel<T, O, int32_t, true>, grid, dim3(threads), shared, stream, a, chunk, chunks);
+    const bool wide = a.history_type == DGNN_I64, many = a.t >= kLongHistory;
+    if (many && wide) return launch_shared(logits_kernel<T, O, int64_t, true, true>, grid, dim3(threads), shared, stream, a, chunk, chunks);
+    if (many) return launch_shared(logits_kernel<T, O, int32_t, true, true>, grid, dim3(threads), shared, stream, a, chunk, chunks);
+    if (wide) return launch_shared(logits_kernel<T, O, int64_t, true, false>, grid, dim3(threads), shared, stream, a, chunk, chunks);
+    return launch_shared(logits_kernel<T, O, int32_t, true, false>, grid, dim3(threads), shared, stream, a, chunk, chunks);
 }
 
 }  // namespace
