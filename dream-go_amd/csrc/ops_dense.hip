@@ -499,6 +499,7 @@ constexpr Form kForms[] = {
 };
 constexpr int kNumForms = sizeof(kForms) / sizeof(kForms[0]), kDirect = -1;
 constexpr double kUnits = 256;
+constexpr int64_t kMaxSplits = 16;
 // One launch more: what it takes on the device and, where calls follow each other closely, the host.
 constexpr double kLaunch = 5.0;
 
@@ -535,9 +536,16 @@ Plan make_plan(const dgnn_dense_args& a)
     for (int f = 0; f < kNumForms; ++f) {
         const Form& form = kForms[f];
         const double count = (double)ceil_div(a.m, form.bm) * (double)ceil_div(a.n, form.bn);
-        for (int64_t splits = 1; splits <= 16; ++splits) {
+        // shares of k where they give idle units something to do, of 256 columns at least
+        int64_t most = 1;
+        if (count * 2 <= kUnits * form.per_unit && a.k >= 512) {
+            most = (int64_t)(kUnits * form.per_unit / count);
+            most = most > a.k / 256 ? a.k / 256 : most;
+            most = most > kMaxSplits ? kMaxSplits : most;
+        }
+        for (int64_t splits = 1; splits <= most; splits = splits < 4 ? splits + 1 : splits + 2) {
             const int64_t share = round_up(ceil_div(a.k, splits), 64);
-            if (splits > 1 && (share < 256 || ceil_div(a.k, share) != splits || count * (double)splits > kUnits * form.per_unit)) continue;
+            if (ceil_div(a.k, share) != splits) continue;
             const double all = count * (double)splits, slots = kUnits * (all <= kUnits ? 1 : form.per_unit);
             const double rounds = (double)(int64_t)((all + slots - 1) / slots), each = (double)(share / 64) * (all <= kUnits ? form.alone : form.crowded) + form.fixed;
             const double join = splits > 1 ? kLaunch + (double)splits * (double)a.m * (double)a.n * 8 / 3.0e6 : 0.0;

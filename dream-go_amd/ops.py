@@ -35,6 +35,7 @@ SYMBOLS = [
 
 ACTIVATIONS = {"identity": 0, "relu": 1, "tanh": 2, "gelu": 3, "silu": 4}
 _TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+_HALVES = {torch.float16: 0, torch.bfloat16: 1}
 _INTEGERS = {torch.int32: 3, torch.int64: 4}
 
 # dgnn_dense_args, dgnn_group_norm_args, dgnn_logits_args
@@ -69,38 +70,56 @@ def _refuse(where, why, status=api.BAD_ARGUMENT):
     raise api.Error(status, f"{where}: {why}")
 
 
-def _tensor(where, name, t, device, types):
-    """The pointer of an operand that lives on `device` and has one of `types`."""
+def _explain(where, name, t, index, types):
+    """Raises what is wrong with an operand that should live on device `index` (None: on any GPU) and have one of `types`."""
     if not isinstance(t, torch.Tensor):
         _refuse(where, f"{name} must be a tensor, got {type(t).__name__}")
-    if t.device != device:
-        _refuse(where, f"{name} is on {t.device}, expected {device}")
-    if t.dtype not in types:
-        _refuse(where, f"{name} is {t.dtype}, expected {' or '.join(str(x) for x in types)}", api.UNSUPPORTED)
-    if t.requires_grad and torch.is_grad_enabled():
-        _refuse(where, f"{name} requires grad: the operators evaluate only (torch.no_grad() or detach())", api.UNSUPPORTED)
-    return t.data_ptr()
+    if not t.is_cuda:
+        _refuse(where, f"{name} must be a tensor on a GPU, it is on {t.device}")
+    if index is not None and t.get_device() != index:
+        _refuse(where, f"{name} is on {t.device}, expected cuda:{index}")
+    _refuse(where, f"{name} is {t.dtype}, expected {' or '.join(str(x) for x in types)}", api.UNSUPPORTED)
+
+
+def _pointer(where, name, t, index, types):
+    """The pointer of an operand; `types` is a dict or tuple of what it may be."""
+    try:
+        if t.get_device() == index and t.dtype in types:
+            return t.data_ptr()
+    except AttributeError:
+        pass
+    _explain(where, name, t, index, types)
 
 
 def _first(where, name, t, types):
-    """The first operand: it says which device the call is for."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        _refuse(where, f"{name} must be a tensor on a GPU")
-    return _tensor(where, name, t, t.device, types)
+    """The device index of the first operand: it says which device the call is for."""
+    try:
+        index = t.get_device()
+        if index >= 0 and t.dtype in types:
+            return index
+    except AttributeError:
+        pass
+    _explain(where, name, t, None, types)
+
+
+def _no_grad(where, **operands):
+    for name, t in operands.items():
+        if isinstance(t, torch.Tensor) and t.requires_grad:
+            _refuse(where, f"{name} requires grad: the operators evaluate only (torch.no_grad() or detach())", api.UNSUPPORTED)
 
 
 def _rows(where, name, t, rows, columns, broadcast=False):
     """The row stride of a [rows, columns] operand whose columns are contiguous; with `broadcast`, [columns] stands for every row."""
     shape = t.shape
-    if broadcast and (shape == (columns,) or shape == (1, columns)):
-        if columns > 1 and t.stride(-1) != 1:
-            _refuse(where, f"{name} must be contiguous in its last dimension", api.UNSUPPORTED)
-        return 0
-    if shape != (rows, columns):
-        _refuse(where, f"{name} is {tuple(shape)}, expected {(rows, columns)}")
-    if columns > 1 and t.stride(1) != 1:
+    if shape == (rows, columns):
+        row, column = t.stride()
+    elif broadcast and (shape == (columns,) or shape == (1, columns)):
+        row, column = 0, t.stride(-1)
+    else:
+        _refuse(where, f"{name} is {tuple(shape)}, expected {(rows, columns)}" + (f" or {(columns,)}" if broadcast else ""))
+    if column != 1 and columns > 1:
         _refuse(where, f"{name} must be contiguous in its last dimension", api.UNSUPPORTED)
-    return t.stride(0) if rows > 1 else columns
+    return row if rows > 1 else columns
 
 
 def _vector(where, name, t, length):
@@ -127,8 +146,29 @@ def _activation(where, name):
     return code
 
 
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+# The current stream of a device as a handle; torch.cuda.current_stream makes an object of it first, which takes as long as a launch.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _stream(index):
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+
+
+def _launch(where, run, workspace, index, block, args):
+    """One call; once more with work memory where it asks for some."""
+    stream = _stream(index)
+    status = run(index, stream, block.pack(*args))
+    if status == 0:
+        return
+    if status == api.BAD_ARGUMENT and workspace is not None:
+        need = ctypes.c_int64()
+        packed = block.pack(*args)
+        if workspace(packed, need) == 0 and need.value:
+            memory = torch.empty(need.value, dtype=torch.uint8, device=torch.device("cuda", index))
+            status = run(index, stream, block.pack(*args[:5], memory.data_ptr(), need.value, *args[7:]))
+            if status == 0:
+                return
+    _fail(status, where)
 
 
 def dense(x, weight, bias=None, residual=None, *, alpha1=1.0, alpha2=1.0, activation="identity", out=None, out_dtype=None):
@@ -142,55 +182,48 @@ def dense(x, weight, bias=None, residual=None, *, alpha1=1.0, alpha2=1.0, activa
     out_dtype x's type (default) or torch.float32
     """
     where = "dense"
-    px = _first(where, "x", x, (torch.float16, torch.bfloat16))
-    device, dtype = x.device, x.dtype
-    pw = _tensor(where, "weight", weight, device, (dtype,))
-    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
-        _refuse(where, f"x {tuple(x.shape)} and weight {tuple(weight.shape)} do not multiply: expected [..., k] and [n, k]")
+    index = _first(where, "x", x, _HALVES)
+    dtype = x.dtype
+    code = _TYPES[dtype]
+    pw = _pointer(where, "weight", weight, index, (dtype,))
+    if torch.is_grad_enabled():
+        _no_grad(where, x=x, weight=weight, bias=bias, residual=residual, out=out)
+    shape = x.shape
+    if not shape or weight.dim() != 2 or shape[-1] != weight.shape[1]:
+        _refuse(where, f"x {tuple(shape)} and weight {tuple(weight.shape)} do not multiply: expected [..., k] and [n, k]")
     n, k = weight.shape
-    leading = x.shape[:-1]
+    leading = shape[:-1]
     m = leading.numel()
-    ldx = _rows(where, "x", _flat(where, "x", x, m), m, k)
-    ldw = _rows(where, "weight", weight, n, k)
+    ldx = k if x.is_contiguous() else _rows(where, "x", _flat(where, "x", x, m), m, k)
+    ldw = k if weight.is_contiguous() else _rows(where, "weight", weight, n, k)
     if out_dtype is None:
         out_dtype = dtype if out is None else out.dtype
-    if out_dtype != dtype and out_dtype != torch.float32:
+    if out_dtype is not dtype and out_dtype is not torch.float32:
         _refuse(where, f"out_dtype {out_dtype} is neither x's type nor torch.float32", api.UNSUPPORTED)
-    pb = pz = ldz = bias_type = 0
+    pb = pz = ldz = 0
+    bias_code = code
     if bias is not None:
-        pb = _tensor(where, "bias", bias, device, (dtype, torch.float32))
+        pb = _pointer(where, "bias", bias, index, (dtype, torch.float32))
         _vector(where, "bias", bias, n)
-        bias_type = _TYPES[bias.dtype]
-    else:
-        bias_type = _TYPES[dtype]
+        bias_code = _TYPES[bias.dtype]
     if residual is not None:
-        pz = _tensor(where, "residual", residual, device, (out_dtype,))
+        pz = _pointer(where, "residual", residual, index, (out_dtype,))
         if residual.dim() == 1:
             _vector(where, "residual", residual, n)
-        elif residual.shape[:-1] != leading:
+        elif residual.shape != (*leading, n):
             _refuse(where, f"residual is {tuple(residual.shape)}, expected {(*leading, n)} or {(n,)}")
         else:
-            ldz = _rows(where, "residual", _flat(where, "residual", residual, m), m, n)
+            ldz = n if residual.is_contiguous() else _rows(where, "residual", _flat(where, "residual", residual, m), m, n)
     if out is None:
-        out = torch.empty(*leading, n, dtype=out_dtype, device=device)
+        out = torch.empty((*leading, n), dtype=out_dtype, device=x.device)
         py, ldy = out.data_ptr(), n
     else:
-        py = _tensor(where, "out", out, device, (out_dtype,))
+        py = _pointer(where, "out", out, index, (out_dtype,))
         if out.shape != (*leading, n):
             _refuse(where, f"out is {tuple(out.shape)}, expected {(*leading, n)}")
-        ldy = _rows(where, "out", _flat(where, "out", out, m), m, n)
-    tail = (m, n, k, ldx, ldw, ldz, ldy, alpha1, alpha2, _TYPES[dtype], _TYPES[out_dtype], bias_type, _activation(where, activation))
-    block = _DENSE.pack(px, pw, pb, pz, py, 0, 0, *tail)
-    need = ctypes.c_int64()
-    status = lib.dgnn_dense_workspace(block, need)
-    if status:
-        _fail(status, where)
-    if need.value:
-        workspace = torch.empty(need.value, dtype=torch.uint8, device=device)
-        block = _DENSE.pack(px, pw, pb, pz, py, workspace.data_ptr(), need.value, *tail)
-    status = lib.dgnn_dense(device.index, _stream(device), block)
-    if status:
-        _fail(status, where)
+        ldy = n if out.is_contiguous() else _rows(where, "out", _flat(where, "out", out, m), m, n)
+    _launch(where, lib.dgnn_dense, lib.dgnn_dense_workspace, index, _DENSE,
+            (x.data_ptr(), pw, pb, pz, py, 0, 0, m, n, k, ldx, ldw, ldz, ldy, alpha1, alpha2, code, _TYPES[out_dtype], bias_code, _activation(where, activation)))
     return out
 
 
@@ -219,55 +252,46 @@ def group_norm(x, num_groups, weight=None, bias=None, residual=None, *, eps=1e-5
     out       of x's shape and type; may be x or residual itself.  Allocated where None
     """
     where = "group_norm"
-    px = _first(where, "x", x, tuple(_TYPES))
-    device, dtype, shape = x.device, x.dtype, x.shape
-    if x.dim() < 2:
+    index = _first(where, "x", x, _TYPES)
+    dtype, shape = x.dtype, x.shape
+    if torch.is_grad_enabled():
+        _no_grad(where, x=x, weight=weight, bias=bias, residual=residual, out=out)
+    if len(shape) < 2:
         _refuse(where, f"x is {tuple(shape)}, expected [n, ..., c]")
     n, c = shape[0], shape[-1]
-    p = shape[1:-1].numel()
-    x_n, x_p = _maps(where, "x", x, shape)
-    num_groups = int(num_groups)
+    p = shape[1] if len(shape) == 3 else shape[1:-1].numel()
+    x_n, x_p = (p * c, c) if x.is_contiguous() else _maps(where, "x", x, shape)
     if num_groups < 1 or c % num_groups:
         _refuse(where, f"{num_groups} groups do not divide {c} channels")
     pw = pb = pz = z_n = z_p = 0
-    affine = None
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None:
-            q = _tensor(where, name, t, device, (dtype, torch.float32) if affine is None else (affine,))
-            _vector(where, name, t, c)
-            affine = t.dtype
-            if name == "weight":
-                pw = q
-            else:
-                pb = q
+    affine = dtype
+    if weight is not None:
+        pw = _pointer(where, "weight", weight, index, (dtype, torch.float32))
+        _vector(where, "weight", weight, c)
+        affine = weight.dtype
+    if bias is not None:
+        pb = _pointer(where, "bias", bias, index, (dtype, torch.float32) if weight is None else (affine,))
+        _vector(where, "bias", bias, c)
+        affine = bias.dtype
     if residual is not None:
-        pz = _tensor(where, "residual", residual, device, (dtype,))
-        z_n, z_p = _maps(where, "residual", residual, shape)
+        pz = _pointer(where, "residual", residual, index, (dtype,))
+        z_n, z_p = (p * c, c) if residual.is_contiguous() and residual.shape == shape else _maps(where, "residual", residual, shape)
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=device)
+        out = torch.empty(shape, dtype=dtype, device=x.device)
         py, y_n, y_p = out.data_ptr(), p * c, c
     else:
-        py = _tensor(where, "out", out, device, (dtype,))
+        py = _pointer(where, "out", out, index, (dtype,))
         y_n, y_p = _maps(where, "out", out, shape)
-    tail = (n, p, c, num_groups, x_n, x_p, z_n, z_p, y_n, y_p, eps, _TYPES[dtype], _TYPES[affine or dtype], _activation(where, activation))
-    block = _GROUP_NORM.pack(px, pw, pb, pz, py, 0, 0, *tail)
-    need = ctypes.c_int64()
-    status = lib.dgnn_group_norm_workspace(block, need)
-    if status:
-        _fail(status, where)
-    if need.value:
-        workspace = torch.empty(need.value, dtype=torch.uint8, device=device)
-        block = _GROUP_NORM.pack(px, pw, pb, pz, py, workspace.data_ptr(), need.value, *tail)
-    status = lib.dgnn_group_norm(device.index, _stream(device), block)
-    if status:
-        _fail(status, where)
+    _launch(where, lib.dgnn_group_norm, lib.dgnn_group_norm_workspace, index, _GROUP_NORM,
+            (x.data_ptr(), pw, pb, pz, py, 0, 0, n, p, c, num_groups, x_n, x_p, z_n, z_p, y_n, y_p, eps, _TYPES[dtype], _TYPES[affine],
+             _activation(where, activation)))
     return out
 
 
-def _per_row(where, name, value, device, rows):
+def _per_row(where, name, value, index, rows):
     """(pointer, value for all) of a penalty: one number, or fp32 [rows]."""
     if isinstance(value, torch.Tensor):
-        p = _tensor(where, name, value, device, (torch.float32,))
+        p = _pointer(where, name, value, index, (torch.float32,))
         _vector(where, name, value, rows)
         return p, 1.0
     return 0, float(value)
@@ -291,52 +315,48 @@ def adjust_logits(logits, *, mask=None, bias=None, history=None, lengths=None, p
     out             [b, v] of the logits' type or fp32; may be logits itself.  Allocated (logits' type) where None
     """
     where = "adjust_logits"
-    pl = _first(where, "logits", logits, tuple(_TYPES))
-    device, dtype = logits.device, logits.dtype
+    index = _first(where, "logits", logits, _TYPES)
+    dtype = logits.dtype
+    if torch.is_grad_enabled():
+        _no_grad(where, logits=logits, bias=bias, repetition=repetition, presence=presence, frequency=frequency, out=out)
     if logits.dim() != 2:
         _refuse(where, f"logits is {tuple(logits.shape)}, expected [b, v]")
     b, v = logits.shape
-    ld_logits = _rows(where, "logits", logits, b, v)
-    pm = ld_mask = pb = ld_bias = ph = t = ld_history = pn = pp = 0
-    bias_type, history_type = _TYPES[dtype], 3
+    ld_logits = v if logits.is_contiguous() else _rows(where, "logits", logits, b, v)
+    pm = ld_mask = pb = ld_bias = ph = t = ld_history = pn = pp = repetitions = presences = frequencies = 0
+    bias_code, history_code = _TYPES[dtype], 3
     if mask is not None:
-        pm = _tensor(where, "mask", mask, device, (torch.int32,))
+        pm = _pointer(where, "mask", mask, index, (torch.int32,))
         ld_mask = _rows(where, "mask", mask, b, (v + 31) // 32, broadcast=True)
     if bias is not None:
-        pb = _tensor(where, "bias", bias, device, (dtype, torch.float32))
+        pb = _pointer(where, "bias", bias, index, (dtype, torch.float32))
         ld_bias = _rows(where, "bias", bias, b, v, broadcast=True)
-        bias_type = _TYPES[bias.dtype]
-    repetitions, repetition = _per_row(where, "repetition", repetition, device, b)
-    presences, presence = _per_row(where, "presence", presence, device, b)
-    frequencies, frequency = _per_row(where, "frequency", frequency, device, b)
+        bias_code = _TYPES[bias.dtype]
+    repetitions, repetition = _per_row(where, "repetition", repetition, index, b)
+    presences, presence = _per_row(where, "presence", presence, index, b)
+    frequencies, frequency = _per_row(where, "frequency", frequency, index, b)
     if history is not None:
-        ph = _tensor(where, "history", history, device, tuple(_INTEGERS))
+        ph = _pointer(where, "history", history, index, _INTEGERS)
         if history.dim() != 2:
             _refuse(where, f"history is {tuple(history.shape)}, expected [b, t]")
         t = history.shape[1]
         ld_history = _rows(where, "history", history, b, t)
-        history_type = _INTEGERS[history.dtype]
-    for name, value in (("lengths", lengths), ("prompt_lengths", prompt_lengths)):
-        if value is not None:
-            if history is None:
-                _refuse(where, f"{name} without history")
-            q = _tensor(where, name, value, device, (torch.int32,))
-            _vector(where, name, value, b)
-            if name == "lengths":
-                pn = q
-            else:
-                pp = q
-    if t == 0:
-        ph = 0
+        history_code = _INTEGERS[history.dtype]
+        if lengths is not None:
+            pn = _pointer(where, "lengths", lengths, index, (torch.int32,))
+            _vector(where, "lengths", lengths, b)
+        if prompt_lengths is not None:
+            pp = _pointer(where, "prompt_lengths", prompt_lengths, index, (torch.int32,))
+            _vector(where, "prompt_lengths", prompt_lengths, b)
+    elif lengths is not None or prompt_lengths is not None:
+        _refuse(where, "lengths without history")
     if out is None:
-        out = torch.empty(b, v, dtype=dtype, device=device)
+        out = torch.empty((b, v), dtype=dtype, device=logits.device)
         po, ld_out, out_dtype = out.data_ptr(), v, dtype
     else:
-        po = _tensor(where, "out", out, device, (dtype, torch.float32))
+        po = _pointer(where, "out", out, index, (dtype, torch.float32))
         ld_out, out_dtype = _rows(where, "out", out, b, v), out.dtype
-    block = _LOGITS.pack(pl, po, pm, pb, ph, pn, pp, repetitions, presences, frequencies, b, v, t, ld_logits, ld_out, ld_mask, ld_bias, ld_history,
-                         repetition, presence, frequency, _TYPES[dtype], _TYPES[out_dtype], bias_type, history_type)
-    status = lib.dgnn_adjust_logits(device.index, _stream(device), block)
-    if status:
-        _fail(status, where)
+    _launch(where, lib.dgnn_adjust_logits, None, index, _LOGITS,
+            (logits.data_ptr(), po, pm, pb, ph if t else 0, pn, pp, repetitions, presences, frequencies, b, v, t, ld_logits, ld_out, ld_mask, ld_bias, ld_history,
+             repetition, presence, frequency, _TYPES[dtype], _TYPES[out_dtype], bias_code, history_code))
     return out
