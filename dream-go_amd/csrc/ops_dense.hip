@@ -135,12 +135,15 @@ __device__ __forceinline__ void dma_row(const char* base, unsigned offset, T* ld
 // A tile is two steps of k = 32.  While the products of one step run, the fragments of the next are read, so a wave never waits for the read
 // it has just asked for; the buffer of a tile is free once its second step has been read, i.e. at the one barrier in the middle of each tile,
 // and is filled again S tiles ahead: a load has S - 1 tiles' products to arrive, and is waited for by count.
+// KG crews of waves share the columns of k tile by tile, each with a ring of its own, and add their sums up in the end: one crew does not ask for as
+// much as a compute unit's path to the L2 carries (32 x 32 outputs: 43 bytes a nanosecond, four crews 52).
+//
 // Rows go from memory into LDS without passing through registers: their addresses and strides are multiples of 16 bytes (dense_pack_kernel sees
 // to it where the caller's are not).  What is left of k behind the last whole tile (masked, element by element) comes FIRST: it is the one tile
 // that is written through registers.
-template <typename T, int FN, int FM, int WN, int WM, int S>
+template <typename T, int FN, int FM, int WN, int WM, int S, int KG>
 struct Tile {
-    static constexpr int kWaves = WN * WM, kThreads = kWaves * 64;
+    static constexpr int kWaves = WN * WM, kThreads = kWaves * KG * 64;         // waves of one crew
     static constexpr int BN = WN * FN * 16, BM = WM * FM * 16, BK = 64;
     static constexpr int kRows = BN + BM;
     static constexpr int kPieces = kRows / 8, kPiecesW = BN / 8;                // 1 KiB pieces (8 rows): first those of W, then those of x
@@ -148,7 +151,7 @@ struct Tile {
     static constexpr int kLoads = (kPieces + kWaves - 1) / kWaves, kLoadsW = kEven ? kPiecesW / kWaves : 0;
     static constexpr int kReads = FN + FM, kProducts = FN * FM;
     static constexpr bool kTied = FN * FM >= 32;
-    static constexpr int kLdsBytes = S * kRows * BK * 2;
+    static constexpr int kLdsBytes = KG * S * kRows * BK * 2;
     static constexpr int kPerUnit = 160 * 1024 / kLdsBytes < 2 ? 1 : 2;         // workgroups on a compute unit at a time
     static_assert(S >= 2 && (S - 2) * kLoads < 64, "loads in flight are counted");
     typedef vec<T, 8> Frag;
@@ -158,7 +161,7 @@ struct Tile {
     const dgnn_dense_args& a;
     T* const lds;                                               // [S][kRows][64]
     int lane;
-    const int wave;
+    const int crew, wave;                                       // the wave's number in its crew
     const int64_t m0, n0;
     const int columns;                                          // of k, from `begin` on
     const char* base_w;
@@ -168,7 +171,8 @@ struct Tile {
     int seg[2];
 
     __device__ __forceinline__ Tile(const dgnn_dense_args& args, T* memory, int64_t m, int64_t n, int64_t begin, int64_t end)
-        : a(args), lds(memory), lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), m0(m), n0(n), columns((int)(end - begin))
+        : a(args), lds(memory + __builtin_amdgcn_readfirstlane(threadIdx.x / (kWaves * 64)) * S * kRows * BK), lane(threadIdx.x & 63),
+          crew(__builtin_amdgcn_readfirstlane(threadIdx.x / (kWaves * 64))), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % kWaves), m0(m), n0(n), columns((int)(end - begin))
     {
         base_w = static_cast<const char*>(a.w) + (n0 * a.ldw + begin) * 2;
         base_x = static_cast<const char*>(a.x) + (m0 * a.ldx + begin) * 2;
@@ -280,24 +284,25 @@ struct Tile {
 
     __device__ __forceinline__ void run(floatx4 (&acc)[FN][FM])
     {
-        const int whole = columns / BK, ragged = columns % BK ? 1 : 0, tiles = whole + ragged;
-        if (tiles == 0) return;
-        // tile t starts at column first + t * 64, the ragged one (t = 0) at the end of the row
-        const int first = ragged ? -BK : 0, filled = tiles < S ? tiles : S;
+        const int whole = columns / BK, more = columns % BK ? 1 : 0, all = whole + more;
+        if (all == 0) return;
+        // tile t of this crew starts at column first + t * KG * 64; the ragged one, the first of all, at the end of the row
+        const int ragged = KG == 1 || crew == 0 ? more : 0, first = (crew - more) * BK, tiles = (all - crew + KG - 1) / KG, turns = (all + KG - 1) / KG;
+        const int filled = tiles < S ? tiles : S;
         __syncthreads();                                        // (the LDS of the tile before)
         for (int t = ragged; t < filled; ++t)
 #pragma unroll
-            for (int j = 0; j < kLoads; ++j) load(j, t, base_w + (int64_t)(first + t * BK) * 2, base_x + (int64_t)(first + t * BK) * 2);
+            for (int j = 0; j < kLoads; ++j) load(j, t, base_w + (int64_t)(first + t * KG * BK) * 2, base_x + (int64_t)(first + t * KG * BK) * 2);
         if (ragged) load_ragged(0, whole * BK);
         wait_for_all_but_tiles<S - 2>(ragged || filled < S ? 0 : S - 2);
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         Frags f0, f1;
 #pragma unroll
-        for (int r = 0; r < kReads; ++r) read(r, 0, 0, f0);
+        for (int r = 0; r < kReads; ++r) read(r, 0, 0, f0);     // (a crew without a tile reads what LDS holds, and uses none of it)
         int t = 0, b = 0;
         for (; t + S < tiles; ++t) {
-            tile<true>(acc, f0, f1, b, 0, first + (t + S) * BK);
+            tile<true>(acc, f0, f1, b, 0, first + (t + S) * KG * BK);
             b = b + 1 == S ? 0 : b + 1;
         }
         for (; t < tiles; ++t) {
@@ -305,6 +310,29 @@ struct Tile {
             b = b + 1 == S ? 0 : b + 1;
         }
         if constexpr (kTied) settle();
+        if constexpr (KG > 1) {
+            for (; t < turns; ++t) __builtin_amdgcn_s_barrier();        // (one barrier in every crew's every turn)
+            join_crews(acc);
+        }
+    }
+
+    // The first crew's sums and the others', in their order.
+    __device__ __forceinline__ void join_crews(floatx4 (&acc)[FN][FM])
+    {
+        static_assert((KG - 1) * kWaves * kProducts * 1024 <= kLdsBytes, "fits the tiles' LDS");
+        floatx4* const place = reinterpret_cast<floatx4*>(lds - crew * S * kRows * BK) + wave * kProducts * 64 + lane;
+        __syncthreads();
+        if (crew > 0) {
+#pragma unroll
+            for (int p = 0; p < kProducts; ++p) place[((crew - 1) * kWaves * kProducts + p) * 64] = acc[p / FM][p % FM];
+        }
+        __syncthreads();
+        if (crew == 0) {
+#pragma unroll 1
+            for (int g = 0; g < KG - 1; ++g)
+#pragma unroll
+                for (int p = 0; p < kProducts; ++p) acc[p / FM][p % FM] += place[(g * kWaves * kProducts + p) * 64];
+        }
     }
 
     // The outputs pass through LDS, 16 rows of the wave's columns at a time, so that each row is written in whole lines.
@@ -315,6 +343,7 @@ struct Tile {
         static_assert(kWaves * 16 * kPitch * sizeof(float) <= S * kRows * BK * sizeof(T), "fits the tiles' LDS");
         float* const mine = reinterpret_cast<float*>(lds) + wave * 16 * kPitch;
         __syncthreads();                                        // every wave has read its last fragments
+        if (crew > 0) return;
 #pragma unroll 1
         for (int j = 0; j < FM; ++j) {
 #pragma unroll
@@ -360,12 +389,12 @@ __device__ __forceinline__ void place(int64_t i, int64_t tiles_m, int64_t tiles_
 }
 
 // `splits` shares of k, of `share` columns (a multiple of 64) each; with more than one, the sums go to `parts`.
-template <typename T, int FN, int FM, int WN, int WM, int S>
-__global__ __launch_bounds__(WN * WM * 64, (WN * WM * Tile<T, FN, FM, WN, WM, S>::kPerUnit + 3) / 4)
+template <typename T, int FN, int FM, int WN, int WM, int S, int KG>
+__global__ __launch_bounds__(WN * WM * KG * 64, (WN * WM * KG * Tile<T, FN, FM, WN, WM, S, KG>::kPerUnit + 3) / 4)
 void dense_tile_kernel(dgnn_dense_args a, int64_t tiles_m, int64_t tiles_n, int64_t splits, int64_t share, float* parts)
 {
-    typedef Tile<T, FN, FM, WN, WM, S> Work;
-    __shared__ __attribute__((aligned(1024))) T lds[S * Work::kRows * Work::BK];
+    typedef Tile<T, FN, FM, WN, WM, S, KG> Work;
+    __shared__ __attribute__((aligned(1024))) T lds[KG * S * Work::kRows * Work::BK];
     const int64_t tiles = tiles_m * tiles_n;
     for (int64_t i = blockIdx.x; i < tiles * splits; i += gridDim.x) {
         const int64_t split = i / tiles, begin = split * share;
@@ -378,29 +407,28 @@ void dense_tile_kernel(dgnn_dense_args a, int64_t tiles_m, int64_t tiles_n, int6
     }
 }
 
-// The shares' sums, in their order, and everything behind them.
+// The shares' sums, in their order, and everything behind them.  Eight columns a thread; the sums of four shares are asked for at a time.
 template <typename T>
 __global__ __launch_bounds__(256)
-void dense_join_kernel(dgnn_dense_args a, int64_t splits, const float* parts)
+void dense_join_kernel(dgnn_dense_args a, int splits, int lanes, const float* parts)
 {
-    const int64_t wide = (a.n + 7) / 8;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.m * wide; i += (int64_t)gridDim.x * 256) {
-        const int64_t m = i / wide, n = i % wide * 8;
-        float v[8] = {};
-        for (int64_t s = 0; s < splits; ++s) {
-            const float* const from = parts + (s * a.m + m) * a.n + n;
-            if (n + 8 <= a.n) {
-                const vec<float, 8> all = load_vec<float, 8>(from);
+    const int lane = threadIdx.x & (lanes - 1), down = 256 / lanes;
+    const int64_t plane = a.m * a.n;
+    for (int64_t m = (int64_t)blockIdx.x * down + threadIdx.x / lanes; m < a.m; m += (int64_t)gridDim.x * down)
+        for (int64_t n = lane * 8; n < a.n; n += lanes * 8) {
+            const float* const from = parts + m * a.n + n;
+            float v[8] = {};
+            for (int s = 0; s < splits; s += 4) {
+                vec<float, 8> four[4];                                         // (behind a row's end: the next one's, and used for nothing)
 #pragma unroll
-                for (int r = 0; r < 8; ++r) v[r] += all[r];
-            } else {
+                for (int q = 0; q < 4; ++q) four[q] = s + q < splits ? load_vec<float, 8>(from + (s + q) * plane) : vec<float, 8>{};
 #pragma unroll
-                for (int r = 0; r < 7; ++r)
-                    if (n + r < a.n) v[r] += from[r];
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) v[r] += four[q][r];
             }
+            finish<T>(a, m, n, v);
         }
-        finish<T>(a, m, n, v);
-    }
 }
 
 // Rows of any alignment -> rows that start at multiples of 16 bytes, zero behind their end.  Sixteen-bit types alone, so their bits.
@@ -410,14 +438,15 @@ struct Packing {
     int64_t rows, ld;
 };
 __global__ __launch_bounds__(256)
-void dense_pack_kernel(Packing w, Packing x, int64_t k, int64_t pitch)
+void dense_pack_kernel(Packing w, Packing x, int64_t k, int64_t pitch, int lanes)
 {
-    const int64_t wide = pitch / 8;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (w.rows + x.rows) * wide; i += (int64_t)gridDim.x * 256) {
-        const int64_t row = i / wide, column = i % wide * 8;
-        const Packing& p = row < w.rows ? w : x;
-        const int64_t r = row < w.rows ? row : row - w.rows;
-        *reinterpret_cast<vec<uint16_t, 8>*>(p.to + r * pitch + column) = load_row<uint16_t>(p.from + r * p.ld, column, k);
+    const int lane = threadIdx.x & (lanes - 1), down = 256 / lanes;
+    for (int64_t row = (int64_t)blockIdx.x * down + threadIdx.x / lanes; row < w.rows + x.rows; row += (int64_t)gridDim.x * down) {
+        const bool of_w = row < w.rows;
+        const int64_t r = of_w ? row : row - w.rows;
+        const uint16_t* const from = (of_w ? w.from : x.from) + r * (of_w ? w.ld : x.ld);
+        uint16_t* const to = (of_w ? w.to : x.to) + r * pitch;
+        for (int64_t column = lane * 8; column < pitch; column += lanes * 8) *reinterpret_cast<vec<uint16_t, 8>*>(to + column) = load_row<uint16_t>(from, column, k);
     }
 }
 
@@ -476,14 +505,14 @@ void dense_direct_kernel(dgnn_dense_args a, int64_t tiles_n, int64_t tiles)
 //
 // A call is priced in every form it could take and takes the cheapest.  The prices are measured (microseconds, bf16): one tile of 64 columns
 // of k where a compute unit holds one workgroup, the same where it holds two, and what a workgroup takes besides (first loads, outputs).  What
-// a form costs beside its neighbours, at the sizes where they change places:
+// the forms cost beside each other at the sizes where they change places (m, k, n; operands not in the caches):
 //   16 x 4096 x 16384 (m, k, n)   direct 36.2   16 x 64: 24.9   32 x 32: 25.4
-//    1 x 2888 x 362               direct  6.4   32 x 32: 11.4
-//   64 x 4096 x 4096              32 x 32: 14.1   64 x 64: 22.5   64 x 128: 31.2
-//   64 x 4096 x 16384             32 x 32: 38.5   64 x 64: 28.4   64 x 128: 33.8
-//  512 x 4096 x 4096              64 x 64: 35.7   64 x 128: 31.5   128 x 128: 39.6   256 x 256: 98.9
-// 4096 x 4096 x 1024              64 x 128: 58.7   128 x 128: 41.4   256 x 256: 107
-// 4096 x 1024 x 4096              128 x 128: 53.4   256 x 256: 38.4
+//    1 x 2888 x 362               direct  6.2   32 x 32:  8.0   64 x 64: 8.5 (shares of k)
+//  256 x 2888 x 362               32 x 32: 12.8   four crews: 11.4   64 x 64: 12.7   64 x 128: 14.8
+// 1024 x 4096 x 1024              64 x 64: 19.4   two crews: 17.0   64 x 128: 19.7   128 x 128: 24.0
+//  512 x 4096 x 4096              64 x 64: 35.8   64 x 128: 31.7   128 x 128: 32.7   256 x 256: 45.4
+// 4096 x 4096 x 1024              64 x 64: 62.4   64 x 128: 59.0   128 x 128: 42.4   256 x 256: 61.1
+// 4096 x 1024 x 4096              64 x 128: 74.8   128 x 128: 53.9   256 x 256: 38.7
 struct Form {
     int bm, bn, per_unit;
     double alone, crowded, fixed;
@@ -491,11 +520,13 @@ struct Form {
 constexpr Form kForms[] = {
     {16, 64, 2, 0.27, 0.40, 2.5},
     {64, 16, 2, 0.27, 0.40, 2.5},
-    {32, 32, 2, 0.19, 0.29, 2.2},
-    {64, 64, 2, 0.32, 0.48, 3.0},
-    {64, 128, 1, 0.47, 0.47, 3.3},
-    {128, 128, 1, 0.60, 0.60, 4.0},
+    {32, 32, 2, 0.19, 0.29, 3.2},
+    {64, 64, 2, 0.30, 0.49, 3.8},
+    {64, 128, 1, 0.47, 0.47, 4.0},
+    {128, 128, 1, 0.60, 0.60, 4.5},
     {256, 256, 1, 1.72, 1.72, 12.0},
+    {32, 32, 1, 0.145, 0.145, 4.6},         // four crews
+    {64, 64, 1, 0.215, 0.215, 4.6},         // two
 };
 constexpr int kNumForms = sizeof(kForms) / sizeof(kForms[0]), kDirect = -1;
 constexpr double kUnits = 256;
@@ -546,8 +577,10 @@ Plan make_plan(const dgnn_dense_args& a)
         for (int64_t splits = 1; splits <= most; splits = splits < 4 ? splits + 1 : splits + 2) {
             const int64_t share = round_up(ceil_div(a.k, splits), 64);
             if (ceil_div(a.k, share) != splits) continue;
-            const double all = count * (double)splits, slots = kUnits * (all <= kUnits ? 1 : form.per_unit);
-            const double rounds = (double)(int64_t)((all + slots - 1) / slots), each = (double)(share / 64) * (all <= kUnits ? form.alone : form.crowded) + form.fixed;
+            const double all = count * (double)splits, slots = kUnits * form.per_unit, rounds = (double)(int64_t)((all + slots - 1) / slots);
+            // (the units that hold two workgroups slow down those alone)
+            const double full = all >= slots ? 1.0 : all <= kUnits ? 0.0 : (all - kUnits) / (slots - kUnits);
+            const double each = (double)(share / 64) * (form.alone + (form.crowded - form.alone) * full) + form.fixed;
             const double join = splits > 1 ? kLaunch + (double)splits * (double)a.m * (double)a.n * 8 / 3.0e6 : 0.0;
             const double cost = rounds * each + join + packing;
             if (cost >= price) continue;
@@ -563,17 +596,25 @@ Plan make_plan(const dgnn_dense_args& a)
     best.pitch = pitch;
     best.bytes_w = best.pack_w ? round_up(a.n * pitch * 2, 256) : 0;
     best.bytes_x = best.pack_x ? round_up(a.m * pitch * 2, 256) : 0;
-    best.bytes_parts = best.splits > 1 ? best.splits * a.m * a.n * 4 : 0;
+    best.bytes_parts = best.splits > 1 ? best.splits * a.m * a.n * 4 + 32 : 0;      // (the last row is read by eights)
     return best;
 }
 
-template <typename T, int FN, int FM, int WN, int WM, int S>
+template <typename T, int FN, int FM, int WN, int WM, int S, int KG>
 hipError_t launch_tiles(const dgnn_dense_args& a, const Plan& plan, float* parts, hipStream_t stream)
 {
-    typedef Tile<T, FN, FM, WN, WM, S> Work;
+    typedef Tile<T, FN, FM, WN, WM, S, KG> Work;
     const int64_t tiles_m = ceil_div(a.m, Work::BM), tiles_n = ceil_div(a.n, Work::BN), all = tiles_m * tiles_n * plan.splits;
-    return launch(dense_tile_kernel<T, FN, FM, WN, WM, S>, dim3((unsigned)(all < kMaxGrid ? all : kMaxGrid)), dim3(Work::kThreads), stream,
+    return launch(dense_tile_kernel<T, FN, FM, WN, WM, S, KG>, dim3((unsigned)(all < kMaxGrid ? all : kMaxGrid)), dim3(Work::kThreads), stream,
                   a, tiles_m, tiles_n, plan.splits, plan.share, parts);
+}
+
+// Threads side by side on a row of `columns`, eight to each: a power of two, a workgroup at most.
+int lanes_for(int64_t columns)
+{
+    int lanes = 1;
+    while (lanes < 256 && lanes * 8 < columns) lanes *= 2;
+    return lanes;
 }
 
 template <typename T>
@@ -595,8 +636,9 @@ hipError_t launch_typed(dgnn_dense_args a, hipStream_t stream)
     if (plan.pack_w || plan.pack_x) {
         const Packing w{static_cast<const uint16_t*>(a.w), reinterpret_cast<uint16_t*>(memory), plan.pack_w ? a.n : 0, a.ldw};
         const Packing x{static_cast<const uint16_t*>(a.x), reinterpret_cast<uint16_t*>(memory + plan.bytes_w), plan.pack_x ? a.m : 0, a.ldx};
-        const int64_t blocks = ceil_div((w.rows + x.rows) * (plan.pitch / 8), 256);
-        const hipError_t err = launch(dense_pack_kernel, dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), stream, w, x, a.k, plan.pitch);
+        const int lanes = lanes_for(plan.pitch);
+        const int64_t blocks = ceil_div(w.rows + x.rows, 256 / lanes);
+        const hipError_t err = launch(dense_pack_kernel, dim3((unsigned)(blocks < kMaxGrid ? blocks : kMaxGrid)), dim3(256), stream, w, x, a.k, plan.pitch, lanes);
         if (err != hipSuccess) return err;
         if (plan.pack_w) { a.w = w.to; a.ldw = plan.pitch; }
         if (plan.pack_x) { a.x = x.to; a.ldx = plan.pitch; }
@@ -604,17 +646,20 @@ hipError_t launch_typed(dgnn_dense_args a, hipStream_t stream)
     }
     hipError_t err = hipErrorInvalidValue;
     switch (plan.form) {
-    case 0: err = launch_tiles<T, 1, 1, 4, 1, 8>(a, plan, parts, stream); break;
-    case 1: err = launch_tiles<T, 1, 1, 1, 4, 8>(a, plan, parts, stream); break;
-    case 2: err = launch_tiles<T, 1, 1, 2, 2, 8>(a, plan, parts, stream); break;
-    case 3: err = launch_tiles<T, 2, 2, 2, 2, 4>(a, plan, parts, stream); break;
-    case 4: err = launch_tiles<T, 4, 2, 2, 2, 4>(a, plan, parts, stream); break;
-    case 5: err = launch_tiles<T, 4, 2, 2, 4, 4>(a, plan, parts, stream); break;
-    case 6: err = launch_tiles<T, 4, 8, 4, 2, 2>(a, plan, parts, stream); break;
+    case 0: err = launch_tiles<T, 1, 1, 4, 1, 8, 1>(a, plan, parts, stream); break;
+    case 1: err = launch_tiles<T, 1, 1, 1, 4, 8, 1>(a, plan, parts, stream); break;
+    case 2: err = launch_tiles<T, 1, 1, 2, 2, 8, 1>(a, plan, parts, stream); break;
+    case 3: err = launch_tiles<T, 2, 2, 2, 2, 4, 1>(a, plan, parts, stream); break;
+    case 4: err = launch_tiles<T, 4, 2, 2, 2, 4, 1>(a, plan, parts, stream); break;
+    case 5: err = launch_tiles<T, 4, 2, 2, 4, 4, 1>(a, plan, parts, stream); break;
+    case 6: err = launch_tiles<T, 4, 8, 4, 2, 2, 1>(a, plan, parts, stream); break;
+    case 7: err = launch_tiles<T, 1, 1, 2, 2, 4, 4>(a, plan, parts, stream); break;
+    case 8: err = launch_tiles<T, 2, 2, 2, 2, 4, 2>(a, plan, parts, stream); break;
     }
     if (err != hipSuccess || !parts) return err;
-    const int64_t blocks = ceil_div(a.m * ceil_div(a.n, 8), 256);
-    return launch(dense_join_kernel<T>, dim3((unsigned)(blocks < kMaxGrid ? blocks : kMaxGrid)), dim3(256), stream, a, plan.splits, parts);
+    const int lanes = lanes_for(a.n);
+    const int64_t blocks = ceil_div(a.m, 256 / lanes);
+    return launch(dense_join_kernel<T>, dim3((unsigned)(blocks < kMaxGrid ? blocks : kMaxGrid)), dim3(256), stream, a, (int)plan.splits, lanes, parts);
 }
 
 }  // namespace
