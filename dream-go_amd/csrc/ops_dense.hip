@@ -506,7 +506,8 @@ void dense_direct_kernel(dgnn_dense_args a, int64_t tiles_n, int64_t tiles)
 // A call is priced in every form it could take and takes the cheapest.  The prices are measured (microseconds, bf16): one tile of 64 columns
 // of k where a compute unit holds one workgroup, the same where it holds two, and what a workgroup takes besides (first loads, outputs).  What
 // the forms cost beside each other at the sizes where they change places (m, k, n; operands not in the caches):
-//   16 x 4096 x 16384 (m, k, n)   direct 36.2   16 x 64: 24.9   32 x 32: 25.4
+//    1 x 4096 x 16384 (m, k, n)   direct 27.5 (4.9 TB/s)   16 x 64: 31.2   32 x 32: 34.4
+//   16 x 4096 x 16384             direct 39.7   16 x 64: 31.2 (4.3 TB/s)   32 x 32: 35.5
 //    1 x 2888 x 362               direct  6.2   32 x 32:  8.0   64 x 64: 8.5 (shares of k)
 //  256 x 2888 x 362               32 x 32: 12.8   four crews: 11.4   64 x 64: 12.7   64 x 128: 14.8
 // 1024 x 4096 x 1024              64 x 64: 19.4   two crews: 17.0   64 x 128: 19.7   128 x 128: 24.0
@@ -556,7 +557,9 @@ Plan make_plan(const dgnn_dense_args& a)
     const bool ready_w = fetchable(a.w, a.ldw, a.n), ready_x = fetchable(a.x, a.ldx, a.m);
     // fragments straight from memory: bound by what a unit's L1 passes on; rows that are not there cost nothing, unaligned ones nearly twice
     const double few = (double)(a.m < a.n ? a.m : a.n), tiles = (double)ceil_div(a.m, 16) * (double)ceil_div(a.n, 16);
-    double price = (tiles > kUnits ? tiles / kUnits : 1.0) * (double)tiles_k * (0.08 + 0.066 * (few < 16 ? few : 16) / 16) * (ready_w && ready_x ? 1.0 : 1.9) + 3.0;
+    const double bytes = ((double)a.m + (double)a.n) * (double)a.k * 2;
+    double price = (tiles > kUnits ? tiles / kUnits : 1.0) * (double)tiles_k * (0.08 + 0.066 * (few < 16 ? few : 16) / 16) * (ready_w && ready_x ? 1.0 : 1.9);
+    price = (price > bytes / 5.0e6 ? price : bytes / 5.0e6) + 3.0;
     if (a.k == 0) return best;
     double packing = 0.0;
     const int64_t pitch = round_up(a.k, 64);
@@ -582,7 +585,7 @@ Plan make_plan(const dgnn_dense_args& a)
             const double full = all >= slots ? 1.0 : all <= kUnits ? 0.0 : (all - kUnits) / (slots - kUnits);
             const double each = (double)(share / 64) * (form.alone + (form.crowded - form.alone) * full) + form.fixed;
             const double join = splits > 1 ? kLaunch + (double)splits * (double)a.m * (double)a.n * 8 / 3.0e6 : 0.0;
-            const double cost = rounds * each + join + packing;
+            const double work = rounds * each, cost = (work > bytes / 4.4e6 ? work : bytes / 4.4e6) + join + packing;
             if (cost >= price) continue;
             price = cost;
             best.form = f;

@@ -237,8 +237,6 @@ void one_pass_kernel(dgnn_group_norm_args a, Layout l)
             load_rows<T, R, V, TINY>(x, l.rows * a.x_p, here, p, held);
             if constexpr (SKIP) load_rows<T, R, V, TINY>(static_cast<const T*>(a.z) + i * a.z_n + p.row * a.z_p + p.c, l.rows * a.z_p, here, p, skip);
             float weight[V], bias[V], sum[V] = {}, mean[V], scale[V];
-            load_affine<T, V>(a.weight, a.affine_type == DGNN_F32, p, 1.0f, weight);
-            load_affine<T, V>(a.bias, a.affine_type == DGNN_F32, p, 0.0f, bias);
 #pragma unroll
             for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -261,6 +259,8 @@ void one_pass_kernel(dgnn_group_norm_args a, Layout l)
 #pragma unroll
             for (int e = 0; e < V; ++e) sum[e] = e < p.n ? sum[e] : 0.0f;
             group_sums<V>(l, p, sum, scratch[1], scales, [&](float s) { return 1.0f / sqrtf(__builtin_fmaf(s, inverse, a.eps)); });
+            load_affine<T, V>(a.weight, a.affine_type == DGNN_F32, p, 1.0f, weight);
+            load_affine<T, V>(a.bias, a.affine_type == DGNN_F32, p, 0.0f, bias);
             of_channels<V>(l, p, scales, scale);
 #pragma unroll
             for (int e = 0; e < V; ++e) scale[e] *= weight[e];

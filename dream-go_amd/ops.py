@@ -102,10 +102,17 @@ def _first(where, name, t, types):
     _explain(where, name, t, None, types)
 
 
-def _no_grad(where, **operands):
-    for name, t in operands.items():
-        if isinstance(t, torch.Tensor) and t.requires_grad:
-            _refuse(where, f"{name} requires grad: the operators evaluate only (torch.no_grad() or detach())", api.UNSUPPORTED)
+def _records(*operands):
+    """Whether gradients are being recorded and one of the operands asks for its own."""
+    if torch.is_grad_enabled():
+        for t in operands:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
+def _no_grad(where):
+    _refuse(where, "an operand requires grad: the operators evaluate only (torch.no_grad() or detach())", api.UNSUPPORTED)
 
 
 def _rows(where, name, t, rows, columns, broadcast=False):
@@ -186,8 +193,6 @@ def dense(x, weight, bias=None, residual=None, *, alpha1=1.0, alpha2=1.0, activa
     dtype = x.dtype
     code = _TYPES[dtype]
     pw = _pointer(where, "weight", weight, index, (dtype,))
-    if torch.is_grad_enabled():
-        _no_grad(where, x=x, weight=weight, bias=bias, residual=residual, out=out)
     shape = x.shape
     if not shape or weight.dim() != 2 or shape[-1] != weight.shape[1]:
         _refuse(where, f"x {tuple(shape)} and weight {tuple(weight.shape)} do not multiply: expected [..., k] and [n, k]")
@@ -222,6 +227,8 @@ def dense(x, weight, bias=None, residual=None, *, alpha1=1.0, alpha2=1.0, activa
         if out.shape != (*leading, n):
             _refuse(where, f"out is {tuple(out.shape)}, expected {(*leading, n)}")
         ldy = n if out.is_contiguous() else _rows(where, "out", _flat(where, "out", out, m), m, n)
+    if _records(x, weight, bias, residual, out):
+        _no_grad(where)
     _launch(where, lib.dgnn_dense, lib.dgnn_dense_workspace, index, _DENSE,
             (x.data_ptr(), pw, pb, pz, py, 0, 0, m, n, k, ldx, ldw, ldz, ldy, alpha1, alpha2, code, _TYPES[out_dtype], bias_code, _activation(where, activation)))
     return out
@@ -254,8 +261,6 @@ def group_norm(x, num_groups, weight=None, bias=None, residual=None, *, eps=1e-5
     where = "group_norm"
     index = _first(where, "x", x, _TYPES)
     dtype, shape = x.dtype, x.shape
-    if torch.is_grad_enabled():
-        _no_grad(where, x=x, weight=weight, bias=bias, residual=residual, out=out)
     if len(shape) < 2:
         _refuse(where, f"x is {tuple(shape)}, expected [n, ..., c]")
     n, c = shape[0], shape[-1]
@@ -277,11 +282,13 @@ def group_norm(x, num_groups, weight=None, bias=None, residual=None, *, eps=1e-5
         pz = _pointer(where, "residual", residual, index, (dtype,))
         z_n, z_p = (p * c, c) if residual.is_contiguous() and residual.shape == shape else _maps(where, "residual", residual, shape)
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=x.device)
+        out = torch.empty_like(x) if x.is_contiguous() else torch.empty(shape, dtype=dtype, device=x.device)
         py, y_n, y_p = out.data_ptr(), p * c, c
     else:
         py = _pointer(where, "out", out, index, (dtype,))
         y_n, y_p = _maps(where, "out", out, shape)
+    if _records(x, weight, bias, residual, out):
+        _no_grad(where)
     _launch(where, lib.dgnn_group_norm, lib.dgnn_group_norm_workspace, index, _GROUP_NORM,
             (x.data_ptr(), pw, pb, pz, py, 0, 0, n, p, c, num_groups, x_n, x_p, z_n, z_p, y_n, y_p, eps, _TYPES[dtype], _TYPES[affine],
              _activation(where, activation)))
@@ -317,8 +324,6 @@ def adjust_logits(logits, *, mask=None, bias=None, history=None, lengths=None, p
     where = "adjust_logits"
     index = _first(where, "logits", logits, _TYPES)
     dtype = logits.dtype
-    if torch.is_grad_enabled():
-        _no_grad(where, logits=logits, bias=bias, repetition=repetition, presence=presence, frequency=frequency, out=out)
     if logits.dim() != 2:
         _refuse(where, f"logits is {tuple(logits.shape)}, expected [b, v]")
     b, v = logits.shape
@@ -332,6 +337,7 @@ def adjust_logits(logits, *, mask=None, bias=None, history=None, lengths=None, p
         pb = _pointer(where, "bias", bias, index, (dtype, torch.float32))
         ld_bias = _rows(where, "bias", bias, b, v, broadcast=True)
         bias_code = _TYPES[bias.dtype]
+    tensors = [t for t in (repetition, presence, frequency) if isinstance(t, torch.Tensor)]
     repetitions, repetition = _per_row(where, "repetition", repetition, index, b)
     presences, presence = _per_row(where, "presence", presence, index, b)
     frequencies, frequency = _per_row(where, "frequency", frequency, index, b)
@@ -351,11 +357,13 @@ def adjust_logits(logits, *, mask=None, bias=None, history=None, lengths=None, p
     elif lengths is not None or prompt_lengths is not None:
         _refuse(where, "lengths without history")
     if out is None:
-        out = torch.empty((b, v), dtype=dtype, device=logits.device)
+        out = torch.empty_like(logits) if logits.is_contiguous() else torch.empty((b, v), dtype=dtype, device=logits.device)
         po, ld_out, out_dtype = out.data_ptr(), v, dtype
     else:
         po = _pointer(where, "out", out, index, (dtype, torch.float32))
         ld_out, out_dtype = _rows(where, "out", out, b, v), out.dtype
+    if _records(logits, bias, out) or (repetitions or presences or frequencies) and _records(*tensors):
+        _no_grad(where)
     _launch(where, lib.dgnn_adjust_logits, None, index, _LOGITS,
             (logits.data_ptr(), po, pm, pb, ph if t else 0, pn, pp, repetitions, presences, frequencies, b, v, t, ld_logits, ld_out, ld_mask, ld_bias, ld_history,
              repetition, presence, frequency, _TYPES[dtype], _TYPES[out_dtype], bias_code, history_code))
