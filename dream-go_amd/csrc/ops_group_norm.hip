@@ -371,7 +371,7 @@ template <typename T, Kind K, bool SKIP, bool TINY>
 __global__ __launch_bounds__(kMaxThreads / 2, 4)
 void apply_kernel(dgnn_group_norm_args a, Layout l, const Moments* moments)
 {
-    constexpr int V = width_of<T>, R = kRegisters / 2;
+    constexpr int V = width_of<T>, R = 2;
     __shared__ float means[kMaxGroups], scales[kMaxGroups];
     const int64_t begin = blockIdx.y * l.share, end = begin + l.share < a.p ? begin + l.share : a.p;
     const int pieces = l.shares * l.subs, waves = (int)(blockDim.x + 63) >> 6;

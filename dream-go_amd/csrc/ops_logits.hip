@@ -25,32 +25,55 @@ __device__ __forceinline__ vec<float, 8> load_eight(const T* p)
     return __builtin_convertvector(load_vec<T, 8>(p), vec<float, 8>);
 }
 
+// The kernel's arguments, read anew: kept from one phase to the next, they and what is made of them are more scalars than there are, and each that
+// is put aside takes vector instructions to fetch.
+typedef const __attribute__((address_space(4))) dgnn_logits_args* Arguments;
+__device__ __forceinline__ Arguments again(Arguments a)
+{
+    asm volatile("" : "+s"(a));
+    return a;
+}
+
+// A row's part of a chunk, as pointers.
+template <typename T, typename O>
+struct Chunk {
+    const T* logits;
+    O* out;
+    const uint8_t* mask;
+    const char* bias;
+    bool bias_is_float;
+    __device__ __forceinline__ Chunk(Arguments a, int64_t i, int64_t v0)
+        : logits(static_cast<const T*>(a->logits) + i * a->ld_logits + v0), out(static_cast<O*>(a->out) + i * a->ld_out + v0),
+          mask(a->mask ? reinterpret_cast<const uint8_t*>(a->mask + i * a->ld_mask) + (v0 >> 3) : nullptr), bias(nullptr), bias_is_float(a->bias_type == DGNN_F32)
+    {
+        if (a->bias) bias = static_cast<const char*>(a->bias) + (i * a->ld_bias + v0) * (bias_is_float ? 4 : (int)sizeof(T));
+    }
+};
+
 // HISTORY: H is the type of its tokens.
 template <typename T, typename O, typename H, bool HISTORY, bool LONG>
 __global__ __launch_bounds__(1024, 8)                   // two workgroups on a unit: one counts while the other writes
-void logits_kernel(dgnn_logits_args a, int chunk, int chunks)
+void logits_kernel(dgnn_logits_args, int chunk, int chunks)
 {
+    const Arguments args = (Arguments)__builtin_amdgcn_kernarg_segment_ptr();   // (the first parameter)
     extern __shared__ __attribute__((aligned(16))) unsigned seen[];             // [chunk] with HISTORY
-    const bool bias_is_float = a.bias_type == DGNN_F32;
-    for (int64_t i = blockIdx.y; i < a.b; i += gridDim.y)
+    for (int64_t i = blockIdx.y; i < args->b; i += gridDim.y)
         for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
             const int64_t v0 = (int64_t)c * chunk;
-            const int n = (int)(a.v - v0 < chunk ? a.v - v0 : chunk);
-            const T* const logits = static_cast<const T*>(a.logits) + i * a.ld_logits + v0;
-            const uint8_t* const mask = a.mask ? reinterpret_cast<const uint8_t*>(a.mask + i * a.ld_mask) + (v0 >> 3) : nullptr;
-            const char* const bias = a.bias ? static_cast<const char*>(a.bias) + (i * a.ld_bias + v0) * (bias_is_float ? 4 : (int)sizeof(T)) : nullptr;
-            O* const out = static_cast<O*>(a.out) + i * a.ld_out + v0;
+            const int64_t left = again(args)->v - v0;
+            const int n = left < chunk ? (int)left : chunk;
             vec<T, 8> held[kEach];
             unsigned allowed[kEach];
             const auto fetch = [&](int base) {
+                const Chunk<T, O> at(again(args), i, v0);
 #pragma unroll
                 for (int q = 0; q < kEach; ++q) {
                     const int e = base + (q * (int)blockDim.x + (int)threadIdx.x) * 8;
                     held[q] = vec<T, 8>{};
                     allowed[q] = 0xff;
                     if (e + 8 <= n) {
-                        held[q] = load_vec<T, 8>(logits + e);
-                        if (mask) allowed[q] = mask[e >> 3];
+                        held[q] = load_vec<T, 8>(at.logits + e);
+                        if (at.mask) allowed[q] = at.mask[e >> 3];
                     }
                 }
             };
@@ -58,24 +81,22 @@ void logits_kernel(dgnn_logits_args a, int chunk, int chunks)
 
             float repetition = 1.0f, inverse = 1.0f, presence = 0.0f, frequency = 0.0f;
             if constexpr (HISTORY) {
-                repetition = a.repetition ? a.repetition[i] : a.repetition_all;
-                inverse = 1.0f / repetition;
-                presence = a.presence ? a.presence[i] : a.presence_all;
-                frequency = a.frequency ? a.frequency[i] : a.frequency_all;
-                const int t = (int)a.t;
-                int length = a.lengths ? a.lengths[i] : t, prompt = a.prompt_lengths ? a.prompt_lengths[i] : 0;
+                const Arguments a = again(args);
+                const int t = (int)a->t;
+                int length = a->lengths ? a->lengths[i] : t, prompt = a->prompt_lengths ? a->prompt_lengths[i] : 0;
                 length = length < 0 ? 0 : length > t ? t : length;
                 __syncthreads();                                               // (seen of the chunk before)
                 for (int e = threadIdx.x * 4; e < chunk; e += blockDim.x * 4) *reinterpret_cast<vec<unsigned, 4>*>(seen + e) = vec<unsigned, 4>{};
                 __syncthreads();
-                const H* const history = static_cast<const H*>(a.history) + i * a.ld_history;
+                const H* const history = static_cast<const H*>(a->history) + i * a->ld_history;
                 const auto note = [&](H token, int e) {
-                    const auto at = (std::make_unsigned_t<H>)(token - (H)v0);      // (v0 < 2^31; a token below it becomes a large number)
+                    typedef std::make_unsigned_t<H> Unsigned;
+                    const Unsigned at = (Unsigned)token - (Unsigned)v0;            // (a token in front of the chunk becomes a large number)
                     if (LONG && e < prompt) {
-                        if (at < (std::make_unsigned_t<H>)n) atomicOr(&seen[at], kPrompt<LONG>);
+                        if (at < (Unsigned)n) atomicOr(&seen[at], kPrompt<LONG>);
                     } else {
                         const unsigned one = e < prompt ? kPrompt<LONG> : 1u;
-                        if (at < (std::make_unsigned_t<H>)n) atomicAdd(&seen[at], one);
+                        if (at < (Unsigned)n) atomicAdd(&seen[at], one);
                     }
                 };
                 const int whole = length & ~3;
@@ -86,6 +107,11 @@ void logits_kernel(dgnn_logits_args a, int chunk, int chunks)
                 }
                 if (whole + (int)threadIdx.x < length) note(history[whole + threadIdx.x], whole + threadIdx.x);
                 __syncthreads();
+                const Arguments p = again(args);
+                repetition = p->repetition ? p->repetition[i] : p->repetition_all;
+                inverse = 1.0f / repetition;
+                presence = p->presence ? p->presence[i] : p->presence_all;
+                frequency = p->frequency ? p->frequency[i] : p->frequency_all;
             }
             const auto penalize = [&](float l, unsigned count) {
                 const unsigned answered = count & kAnswers<LONG>;
@@ -94,6 +120,7 @@ void logits_kernel(dgnn_logits_args a, int chunk, int chunks)
             };
             for (int base = 0; base < n; base += kEach * 8 * blockDim.x) {
                 if (base > 0) fetch(base);
+                const Chunk<T, O> at(again(args), i, v0);
 #pragma unroll
                 for (int q = 0; q < kEach; ++q) {
                     const int e = base + (q * (int)blockDim.x + (int)threadIdx.x) * 8;
@@ -105,18 +132,18 @@ void logits_kernel(dgnn_logits_args a, int chunk, int chunks)
                             for (int r = 0; r < 8; ++r)
                                 if (__builtin_amdgcn_ballot_w64(counts[r] != 0)) l[r] = penalize(l[r], counts[r]);      // (most of a vocabulary is never seen)
                         }
-                        if (bias) l += bias_is_float ? load_eight(reinterpret_cast<const float*>(bias) + e) : load_eight(reinterpret_cast<const T*>(bias) + e);
-                        if (mask) {
+                        if (at.bias) l += at.bias_is_float ? load_eight(reinterpret_cast<const float*>(at.bias) + e) : load_eight(reinterpret_cast<const T*>(at.bias) + e);
+                        if (at.mask) {
 #pragma unroll
                             for (int r = 0; r < 8; ++r) l[r] = allowed[q] & 1u << r ? l[r] : -INFINITY;
                         }
-                        store_vec<O, 8>(out + e, __builtin_convertvector(l, vec<O, 8>));
+                        store_vec<O, 8>(at.out + e, __builtin_convertvector(l, vec<O, 8>));
                     } else {
                         for (int r = e; r < n; ++r) {
-                            float l = (float)logits[r];
+                            float l = (float)at.logits[r];
                             if constexpr (HISTORY) l = penalize(l, seen[r]);
-                            if (bias) l += load_either<T>(bias, r, bias_is_float);
-                            out[r] = (O)(!mask || (mask[r >> 3] >> (r & 7) & 1) ? l : -INFINITY);
+                            if (at.bias) l += load_either<T>(at.bias, r, at.bias_is_float);
+                            at.out[r] = (O)(!at.mask || (at.mask[r >> 3] >> (r & 7) & 1) ? l : -INFINITY);
                         }
                     }
                     __builtin_amdgcn_sched_barrier(0);          // (one vector after the other: together they take more registers than there are)
