@@ -32,10 +32,10 @@ HOST_SOURCES = ["loader.cpp", "network.cpp", "engine.cpp", "rccl.cpp", "batcher.
 KERNEL_SOURCES = ["conv_board.hip", "conv_board_b.hip", "conv_board_tower.hip", "kernels.hip", "heads.hip", "features.hip"]
 OPS_LIB_PATH = os.path.join(HERE, "lib", "libdgnn_ops.so")
 OPS_SOURCES = ["ops.cpp", "ops_dense.hip", "ops_group_norm.hip", "ops_logits.hip"]
-# The operators' kernels use no packed fp32 arithmetic: the compiler forms v_pk_{add,mul,fma}_f32 from plain float code, and some forms
-# have given wrong results on this part.  (The host pass does not know the feature and says so.)
-OPS_FLAGS = ["-fvisibility=hidden", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-result"]
+OPS_FLAGS = ["-fvisibility=hidden"]
+# No packed fp32 arithmetic: the compiler forms v_pk_{add,mul,fma}_f32 from plain float code, and some forms have given wrong results on
+# this part, now and then and without an error.  (The host pass does not know the feature and says so.)
+FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-result", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 if ABLATIONS:
     FLAGS.append("-DDGNN_ABLATIONS")
     KERNEL_SOURCES.append(os.path.join("ablations", "conv_tile.hip"))

@@ -45,7 +45,6 @@ namespace {
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
-typedef float floatx2 __attribute__((ext_vector_type(2)));
 
 constexpr int kRows = kBoardRows;                      // 400 padded rows per board
 constexpr int kHalo = 21;                              // rows above row 0 that a tap can reach (20 + 1)
@@ -1137,13 +1136,7 @@ __device__ __forceinline__ int conv_board_body(const ConvBoardLaunch& a, char* c
                 const half4 z4 = __builtin_bit_cast(half4, kk == 0 ? zx : zy);
                 float t[4];
 #pragma unroll
-                for (int jj = 0; jj < 4; jj += 2) {
-                    // two fp32 fmas per instruction (v_pk_fma_f32: same rounding per element; no MFMA is running beside it here)
-                    const floatx2 av = {acc[c2][rt][jj], acc[c2][rt][jj + 1]}, bv = {bias[c2][jj], bias[c2][jj + 1]}, sv = {a.alpha1, a.alpha1};
-                    const floatx2 tv = __builtin_elementwise_fma(sv, av, bv);
-                    t[jj] = tv[0];
-                    t[jj + 1] = tv[1];
-                }
+                for (int jj = 0; jj < 4; ++jj) t[jj] = __builtin_fmaf(a.alpha1, acc[c2][rt][jj], bias[c2][jj]);
                 if constexpr (SKIP == 1) {
 #pragma unroll
                     for (int jj = 0; jj < 4; ++jj) t[jj] = __builtin_fmaf(a.alpha2, (float)z4[jj], t[jj]);
