@@ -10,6 +10,7 @@ thread_local int g_last_hip_error = 0;
 int hip_failed(hipError_t err)
 {
     g_last_hip_error = (int)err;
+    (void)hipGetLastError();            // the runtime keeps it as well, for whoever asks next: it has been told here
     return DGNN_HIP_ERROR;
 }
 

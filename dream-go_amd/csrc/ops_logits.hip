@@ -82,14 +82,13 @@ void logits_kernel(dgnn_logits_args, int chunk, int chunks)
             float repetition = 1.0f, inverse = 1.0f, presence = 0.0f, frequency = 0.0f;
             if constexpr (HISTORY) {
                 const Arguments a = again(args);
-                const int t = (int)a->t;
-                int length = a->lengths ? a->lengths[i] : t, prompt = a->prompt_lengths ? a->prompt_lengths[i] : 0;
-                length = length < 0 ? 0 : length > t ? t : length;
+                const int t = (int)a->t, wanted = a->lengths ? a->lengths[i] : t, given = a->prompt_lengths ? a->prompt_lengths[i] : 0;
+                const unsigned length = wanted < 0 ? 0 : wanted > t ? t : wanted, prompt = given < 0 ? 0 : given;     // (counting past either stays in 32 bits)
                 __syncthreads();                                               // (seen of the chunk before)
                 for (int e = threadIdx.x * 4; e < chunk; e += blockDim.x * 4) *reinterpret_cast<vec<unsigned, 4>*>(seen + e) = vec<unsigned, 4>{};
                 __syncthreads();
                 const H* const history = static_cast<const H*>(a->history) + i * a->ld_history;
-                const auto note = [&](H token, int e) {
+                const auto note = [&](H token, unsigned e) {
                     typedef std::make_unsigned_t<H> Unsigned;
                     const Unsigned at = (Unsigned)token - (Unsigned)v0;            // (a token in front of the chunk becomes a large number)
                     if (LONG && e < prompt) {
@@ -99,13 +98,13 @@ void logits_kernel(dgnn_logits_args, int chunk, int chunks)
                         if (at < (Unsigned)n) atomicAdd(&seen[at], one);
                     }
                 };
-                const int whole = length & ~3;
-                for (int e = threadIdx.x * 4; e < whole; e += blockDim.x * 4) {
+                const unsigned whole = length & ~3u;
+                for (unsigned e = threadIdx.x * 4; e < whole; e += blockDim.x * 4) {
                     const vec<H, 4> four = load_vec<H, 4>(history + e);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) note(four[r], e + r);
                 }
-                if (whole + (int)threadIdx.x < length) note(history[whole + threadIdx.x], whole + threadIdx.x);
+                if (whole + threadIdx.x < length) note(history[whole + threadIdx.x], whole + threadIdx.x);
                 __syncthreads();
                 const Arguments p = again(args);
                 repetition = p->repetition ? p->repetition[i] : p->repetition_all;

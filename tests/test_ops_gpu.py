@@ -455,6 +455,31 @@ def test_dense_and_group_norm_beyond_two_to_the_31_elements(ops):
     assert torch.equal(ops.group_norm(maps, 4, out=maps), want)
 
 
+def test_more_work_than_one_grid_holds(ops):
+    """Loops behind a capped grid: rows, samples, slabs and sequences beyond what one launch numbers."""
+    g = gen(11)
+    x, w = whole((16_800_000, 8), g, torch.float16).cuda(), whole((3, 8), g, torch.float16).cuda()
+    assert torch.equal(ops.dense(x, w), (x[:, None, :].float() * w.float()).sum(-1).half())
+    group_norm_case(ops, (40000, 3, 16), 2, torch.float16, "relu", torch.float32, True)
+    group_norm_case(ops, (1, 2, 64 * 66000), 66000, torch.float16, "identity", torch.float16)
+    logits = torch.randn(70000, 40, generator=g).cuda()
+    assert torch.equal(ops.adjust_logits(logits, bias=torch.ones(40, device="cuda")), logits + 1)
+    history = torch.arange(70000, dtype=torch.int32, device="cuda")[:, None] % 40
+    want = logits.scatter_add(1, history.long(), torch.full((70000, 1), -0.5, device="cuda"))
+    assert torch.equal(ops.adjust_logits(logits, history=history, frequency=0.5), want)
+
+
+def test_an_error_of_the_runtime_is_told_once(ops, api):
+    x = torch.ones(4, 8, dtype=torch.float16, device="cuda")
+    y = torch.empty(4, 4, dtype=torch.float16, device="cuda")
+    block = ops._DENSE.pack(x.data_ptr(), x.data_ptr(), 0, 0, y.data_ptr(), 0, 0, 4, 4, 8, 8, 8, 0, 4, 1.0, 1.0, 0, 0, 0, 0)
+    assert ops.lib.dgnn_dense(1 << 20, None, block) == api.HIP_ERROR and ops.lib.dgnn_ops_last_hip_error() != 0
+    assert torch.equal(torch.relu(x), x)                                       # torch asks the runtime after its launches
+    assert ops.lib.dgnn_dense(0, None, block) == api.OK
+    torch.cuda.synchronize()
+    assert (y == 8).all()
+
+
 # ---- refusals -----------------------------------------------------------------------------------------------------------------------
 
 def test_refusals_of_the_python_mirror(ops, api):
