@@ -117,13 +117,19 @@ __device__ __forceinline__ float moved(float v)
     return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), Control, 0xf, 0xf, true));
 }
 
-// The sum over a wave, the same in every lane.  Inside a row of sixteen lanes by data-parallel moves, which cost no trip through LDS.
-__device__ __forceinline__ float wave_sum(float v)
+// The sum over a row of sixteen lanes, the same in every one of them: data-parallel moves, which cost no trip through LDS.
+__device__ __forceinline__ float row_sum(float v)
 {
     v += moved<0xb1>(v);                // quad_perm [1, 0, 3, 2]
     v += moved<0x4e>(v);                // quad_perm [2, 3, 0, 1]
     v += moved<0x141>(v);               // row_half_mirror
-    v += moved<0x140>(v);               // row_mirror
+    return v + moved<0x140>(v);         // row_mirror
+}
+
+// The sum over a wave, the same in every lane.
+__device__ __forceinline__ float wave_sum(float v)
+{
+    v = row_sum(v);
     const auto row = [&](int lane) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane)); };
     return (row(0) + row(16)) + (row(32) + row(48));
 }

@@ -8,7 +8,12 @@
 //   two        it does not: a first kernel leaves (mean, sum of squares about it) of every share of the positions, a second joins those of its
 //              groups -- about their joint mean, in a fixed order -- and reads the maps again, mostly out of the last-level cache
 //
-// Bound by memory on both ways; the activations are branch-free for that reason (ops_device.h).
+// Large maps are bound by memory on both ways; the activations are branch-free for that reason (ops_device.h).  256 maps of 361 x 256 fp16 with a
+// skip (142 MB) take 32.5 us in one pass, 4.4 TB/s; 8 maps of 16384 x 320 bf16 with SiLU (168 MB, a third of it read twice) 58 us in two, 2.9 TB/s
+// of what has to move.  Small ones are bound by the chain of waits and by what a thread does beside its values: one map of 361 x 64 takes 5.9 us, of
+// which an empty kernel's launch is about 2.5.  Kernels are made for what a call's sizes promise (Shape) because of the latter: vectors of one
+// group each need one sum where others need eight, whole ones no masks (one map of 361 x 256: 5.8 us, 6.4 without the distinction; 383 maps of
+// 15 x 128: 10.7 us, 20.6 -- that one because LDS is now asked for as needed, not for the largest workgroup).
 #include "ops_device.h"
 
 namespace dgnn {
@@ -22,6 +27,9 @@ constexpr int kUnitsWanted = 256;                                       // workg
 
 template <typename T> constexpr int width_of = 16 / (int)sizeof(T);     // elements of a vector
 
+// What a call's sizes promise its kernels: vectors of one group each; whole vectors; nothing; rows shorter than a vector.
+enum Shape { kAligned, kWhole, kRagged, kTiny };
+
 // How a call is cut up; the same for every workgroup.
 struct Layout {
     int per;                // channels of a group
@@ -32,6 +40,7 @@ struct Layout {
     int threads;
     int shares;             // of a sample's positions
     int64_t share;          // positions of each
+    int scratch;            // floats that group_sums needs
 };
 
 // The part of a slab that a thread works on.
@@ -43,7 +52,7 @@ struct Part {
     int back;               // how far back a whole vector has to begin to end inside the row
 };
 
-template <int V>
+template <Shape S, int V>
 __device__ __forceinline__ Part part_of(const Layout& l, int channels, int groups, int slab)
 {
     Part p;
@@ -68,7 +77,7 @@ __device__ __forceinline__ Part part_of(const Layout& l, int channels, int group
     p.n = p.channels - p.at < V ? p.channels - p.at : V;
     p.row = row < l.rows && p.n > 0 ? row : -1;
     if (p.row < 0) p.at = p.n = 0, p.c = c0;
-    p.back = p.c + V <= channels ? 0 : p.c + V - channels;
+    p.back = S <= kWhole || p.c + V <= channels ? 0 : p.c + V - channels;
     return p;
 }
 
@@ -86,11 +95,11 @@ __device__ __forceinline__ vec<T, V> moved_down(vec<T, V> v, int n)
 }
 
 // The thread's part of `here` rows (R at most), `step` elements apart; zeros behind a part's end and for the other rows.  All loads first, then
-// what makes them parts: the loads of a thread are on their way at once.  TINY: no row is as long as a vector.
-template <typename T, int R, int V, bool TINY>
+// what makes them parts: the loads of a thread are on their way at once.
+template <Shape S, typename T, int R, int V>
 __device__ __forceinline__ void load_rows(const T* p, int64_t step, int here, const Part& part, vec<T, V> (&held)[R])
 {
-    if constexpr (TINY) {
+    if constexpr (S == kTiny) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
 #pragma unroll
@@ -105,7 +114,7 @@ __device__ __forceinline__ void load_rows(const T* p, int64_t step, int here, co
         held[r] = r < here ? load_vec<T, V>(p) : vec<T, V>{};
         p += step;
     }
-    if (part.n < V) {
+    if (S == kRagged && part.n < V) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             if (part.back > 0) held[r] = moved_down<T, V>(held[r], part.back);
@@ -115,25 +124,25 @@ __device__ __forceinline__ void load_rows(const T* p, int64_t step, int here, co
     }
 }
 
-template <typename T, int V>
+template <Shape S, typename T, int V>
 __device__ __forceinline__ void store_part(T* p, int n, const float (&v)[V])
 {
     vec<T, V> out;
 #pragma unroll
     for (int e = 0; e < V; ++e) out[e] = (T)v[e];
-    if (n == V) return store_vec<T, V>(p, out);
+    if (S <= kWhole || n == V) return store_vec<T, V>(p, out);
 #pragma unroll
     for (int e = 0; e < V; ++e)
         if (e < n) p[e] = out[e];
 }
 
-template <typename T, int V>
+template <Shape S, typename T, int V>
 __device__ __forceinline__ void load_affine(const void* from, bool is_float, const Part& p, float otherwise, float (&v)[V])
 {
 #pragma unroll
     for (int e = 0; e < V; ++e) v[e] = otherwise;
     if (!from || p.n <= 0) return;
-    if (p.back == 0) {                                          // (of the channels behind the part nothing is used)
+    if (S <= kWhole || p.back == 0) {                                          // (of the channels behind the part nothing is used)
         if (is_float) {
             const vec<float, V> all = load_vec<float, V>(static_cast<const float*>(from) + p.c);
 #pragma unroll
@@ -151,10 +160,10 @@ __device__ __forceinline__ void load_affine(const void* from, bool is_float, con
 }
 
 // One number of every group of the slab for each channel of the thread's vector.
-template <int V>
+template <Shape S, int V>
 __device__ __forceinline__ void of_channels(const Layout& l, const Part& p, const float* of_group, float (&v)[V])
 {
-    if (l.groups_per_slab == 1 || l.per % V == 0) {
+    if (S == kAligned || (S != kWhole && l.groups_per_slab == 1)) {
         const float all = of_group[l.groups_per_slab == 1 ? 0 : p.at / l.per];
 #pragma unroll
         for (int e = 0; e < V; ++e) v[e] = all;
@@ -170,11 +179,11 @@ __device__ __forceinline__ void of_channels(const Layout& l, const Part& p, cons
 
 // The sums of `mine` over the threads of each group of the slab, as `last` makes them, to out[group].  One barrier inside and one behind;
 // `scratch` is not the one of the call before.
-template <int V, typename Last>
+template <Shape S, int V, typename Last>
 __device__ __forceinline__ void group_sums(const Layout& l, const Part& p, float (&mine)[V], float* scratch, float* out, Last last)
 {
     // a vector, or the whole slab, lies in one group: one number of each thread is enough
-    const bool single = l.groups_per_slab == 1 || l.per % V == 0;
+    const bool single = S == kAligned || (S != kWhole && l.groups_per_slab == 1);
     // rows of a power of two are added up within each wave first
     const bool even = (l.lanes & (l.lanes - 1)) == 0 && l.lanes <= 64;
     const int waves = (int)(blockDim.x + 63) >> 6, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -221,28 +230,30 @@ template <typename V>
 __device__ __forceinline__ void as_loaded(V& v) { asm volatile("" : "+v"(v)); }
 
 // R vectors per thread.
-template <typename T, int R, Kind K, bool SKIP, bool TINY>
+template <Shape S, typename T, int R, Kind K, bool SKIP>
 __global__ __launch_bounds__(R == kRegisters ? kMaxThreads / 2 : kMaxThreads, 4)
 void one_pass_kernel(dgnn_group_norm_args a, Layout l)
 {
     constexpr int V = width_of<T>;
-    __shared__ float scratch[2][kMaxThreads * V], means[kMaxGroups], scales[kMaxGroups];
+    extern __shared__ float scratch[];
+    float* const means = scratch + 2 * l.scratch;
+    float* const scales = means + l.groups_per_slab;
     const float inverse = 1.0f / ((float)a.p * (float)l.per);
     for (int64_t i = blockIdx.z; i < a.n; i += gridDim.z)
         for (int slab = blockIdx.x; slab < l.slabs; slab += gridDim.x) {
-            const Part p = part_of<V>(l, (int)a.c, (int)a.groups, slab);
+            const Part p = part_of<S, V>(l, (int)a.c, (int)a.groups, slab);
             const int here = p.row < 0 || p.row >= a.p ? 0 : (int)(a.p - 1 - p.row) / l.rows + 1;    // positions of this thread
             const T* const x = static_cast<const T*>(a.x) + i * a.x_n + p.row * a.x_p + p.c;
             vec<T, V> held[R], skip[SKIP ? R : 1];
-            load_rows<T, R, V, TINY>(x, l.rows * a.x_p, here, p, held);
-            if constexpr (SKIP) load_rows<T, R, V, TINY>(static_cast<const T*>(a.z) + i * a.z_n + p.row * a.z_p + p.c, l.rows * a.z_p, here, p, skip);
+            load_rows<S, T, R, V>(x, l.rows * a.x_p, here, p, held);
+            if constexpr (SKIP) load_rows<S, T, R, V>(static_cast<const T*>(a.z) + i * a.z_n + p.row * a.z_p + p.c, l.rows * a.z_p, here, p, skip);
             float weight[V], bias[V], sum[V] = {}, mean[V], scale[V];
 #pragma unroll
             for (int r = 0; r < R; ++r)
 #pragma unroll
                 for (int e = 0; e < V; ++e) sum[e] += (float)held[r][e];
-            group_sums<V>(l, p, sum, scratch[0], means, [&](float s) { return s * inverse; });
-            of_channels<V>(l, p, means, mean);
+            group_sums<S, V>(l, p, sum, scratch, means, [&](float s) { return s * inverse; });
+            of_channels<S, V>(l, p, means, mean);
 #pragma unroll
             for (int r = 0; r < R; ++r) as_loaded(held[r]);
 #pragma unroll
@@ -258,10 +269,10 @@ void one_pass_kernel(dgnn_group_norm_args a, Layout l)
                 }
 #pragma unroll
             for (int e = 0; e < V; ++e) sum[e] = e < p.n ? sum[e] : 0.0f;
-            group_sums<V>(l, p, sum, scratch[1], scales, [&](float s) { return 1.0f / sqrtf(__builtin_fmaf(s, inverse, a.eps)); });
-            load_affine<T, V>(a.weight, a.affine_type == DGNN_F32, p, 1.0f, weight);
-            load_affine<T, V>(a.bias, a.affine_type == DGNN_F32, p, 0.0f, bias);
-            of_channels<V>(l, p, scales, scale);
+            group_sums<S, V>(l, p, sum, scratch + l.scratch, scales, [&](float s) { return 1.0f / sqrtf(__builtin_fmaf(s, inverse, a.eps)); });
+            load_affine<S, T, V>(a.weight, a.affine_type == DGNN_F32, p, 1.0f, weight);
+            load_affine<S, T, V>(a.bias, a.affine_type == DGNN_F32, p, 0.0f, bias);
+            of_channels<S, V>(l, p, scales, scale);
 #pragma unroll
             for (int e = 0; e < V; ++e) scale[e] *= weight[e];
 #pragma unroll
@@ -277,7 +288,7 @@ void one_pass_kernel(dgnn_group_norm_args a, Layout l)
                         if constexpr (SKIP) v[e] += (float)skip[r][e];
                     }
                     activate_kind<K>(v, a.activation);
-                    store_part<T, V>(y, p.n, v);
+                    store_part<S, T, V>(y, p.n, v);
                     y += l.rows * a.y_p;
                 }
         }
@@ -294,46 +305,36 @@ struct Moments {
 // look at the values would take six, and this kernel is bound by them as much as by memory.  The shift is one of the n values it is taken from, so
 // n (mean - shift)^2 is less than n times the sum of squares about the mean, whatever the values are: n times a rounding is all that the
 // difference `square - sum^2 / n` can lose.  The threads of a group are then joined about their common mean.
-template <typename T, bool TINY>
+template <Shape S, typename T>
 __global__ __launch_bounds__(kMaxThreads / 2, 4)
 void moments_kernel(dgnn_group_norm_args a, Layout l, Moments* moments)
 {
     constexpr int V = width_of<T>, R = kRegisters;
-    __shared__ float scratch[2][kMaxThreads / 2 * V], means[kMaxGroups], squares[kMaxGroups];
+    extern __shared__ float scratch[];
+    float* const means = scratch + 2 * l.scratch;
+    float* const squares = means + l.groups_per_slab;
     const int64_t begin = blockIdx.y * l.share, end = begin + l.share < a.p ? begin + l.share : a.p;
     for (int64_t i = blockIdx.z; i < a.n; i += gridDim.z)
         for (int slab = blockIdx.x; slab < l.slabs; slab += gridDim.x) {
-            const Part p = part_of<V>(l, (int)a.c, (int)a.groups, slab);
+            const Part p = part_of<S, V>(l, (int)a.c, (int)a.groups, slab);
             const float inverse = 1.0f / ((float)(end - begin) * (float)(l.subs > 1 ? p.channels : l.per));
             const int rows = (int)(end - begin), here = p.row < 0 || p.row >= rows ? 0 : (rows - 1 - p.row) / l.rows + 1;
             float shift[V] = {}, sum[V] = {}, square[V] = {};
             if (here > 0) {
                 const int64_t step = l.rows * a.x_p;
                 const T* x = static_cast<const T*>(a.x) + i * a.x_n + (begin + p.row) * a.x_p + p.c;
-                vec<T, V> first[1];
-                load_rows<T, 1, V, TINY>(x, step, 1, p, first);
-#pragma unroll
-                for (int e = 0; e < V; ++e) shift[e] = (float)first[0][e];
-                int done = 0;
-                for (; done + R <= here; done += R) {
+                for (int done = 0; done < here; done += R) {
+                    const int now = here - done < R ? here - done : R;
                     vec<T, V> held[R];
-                    load_rows<T, R, V, TINY>(x, step, R, p, held);
+                    load_rows<S, T, R, V>(x, step, now, p, held);
                     x += R * step;
+                    if (done == 0) {
+#pragma unroll
+                        for (int e = 0; e < V; ++e) shift[e] = (float)held[0][e];
+                    }
 #pragma unroll
                     for (int r = 0; r < R; ++r)
-#pragma unroll
-                        for (int e = 0; e < V; ++e) {
-                            const float d = (float)held[r][e] - shift[e];
-                            sum[e] += d;
-                            square[e] = __builtin_fmaf(d, d, square[e]);
-                        }
-                }
-                if (done < here) {
-                    vec<T, V> held[R];
-                    load_rows<T, R, V, TINY>(x, step, here - done, p, held);
-#pragma unroll
-                    for (int r = 0; r < R; ++r)
-                        if (done + r < here) {
+                        if (r < now) {
 #pragma unroll
                             for (int e = 0; e < V; ++e) {
                                 const float d = (float)held[r][e] - shift[e];
@@ -353,98 +354,141 @@ void moments_kernel(dgnn_group_norm_args a, Layout l, Moments* moments)
                 mean[e] = shift[e] + about;
                 mine[e] = e < p.n ? mean[e] * count : 0.0f;
             }
-            group_sums<V>(l, p, mine, scratch[0], means, [&](float s) { return s * inverse; });
-            of_channels<V>(l, p, means, joint);
+            group_sums<S, V>(l, p, mine, scratch, means, [&](float s) { return s * inverse; });
+            of_channels<S, V>(l, p, means, joint);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 const float d = mean[e] - joint[e];
                 mine[e] = e < p.n ? __builtin_fmaf(d * d, count, square[e]) : 0.0f;
             }
-            group_sums<V>(l, p, mine, scratch[1], squares, [&](float s) { return s; });
+            group_sums<S, V>(l, p, mine, scratch + l.scratch, squares, [&](float s) { return s; });
             for (int g = threadIdx.x; g < p.groups; g += blockDim.x)
                 moments[((i * a.groups + p.g0 + g) * l.shares + blockIdx.y) * l.subs + p.sub] = Moments{means[g], squares[g]};
             __syncthreads();                                    // (means and squares are the next slab's)
         }
 }
 
-template <typename T, Kind K, bool SKIP, bool TINY>
+template <Shape S, typename T, Kind K, bool SKIP>
 __global__ __launch_bounds__(kMaxThreads / 2, 4)
 void apply_kernel(dgnn_group_norm_args a, Layout l, const Moments* moments)
 {
     constexpr int V = width_of<T>, R = 2;
     __shared__ float means[kMaxGroups], scales[kMaxGroups];
     const int64_t begin = blockIdx.y * l.share, end = begin + l.share < a.p ? begin + l.share : a.p;
-    const int pieces = l.shares * l.subs, waves = (int)(blockDim.x + 63) >> 6;
+    constexpr int G = 2, Q = 4;
+    const int pieces = l.shares * l.subs, waves = (int)(blockDim.x + 63) >> 6, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const auto count = [&](int piece) {                         // values of a piece
+        int share = piece, wide = l.per;
+        if (l.subs > 1) {
+            share = piece / l.subs;
+            const int from = (piece - share * l.subs) * kMaxVectors * V;
+            wide = l.per - from < kMaxVectors * V ? l.per - from : kMaxVectors * V;
+        }
+        return (float)(share < l.shares - 1 ? l.share : a.p - (l.shares - 1) * l.share) * (float)wide;
+    };
     const float inverse = 1.0f / ((float)a.p * (float)l.per);
     for (int64_t i = blockIdx.z; i < a.n; i += gridDim.z)
         for (int slab = blockIdx.x; slab < l.slabs; slab += gridDim.x) {
-            const Part p = part_of<V>(l, (int)a.c, (int)a.groups, slab);
-            for (int g = threadIdx.x >> 6; g < p.groups; g += waves) {
-                const Moments* const of = moments + (i * a.groups + p.g0 + g) * pieces;
-                const auto count = [&](int piece) {
-                    const int share = piece / l.subs, from = (piece - share * l.subs) * kMaxVectors * V;
-                    const int64_t left = a.p - share * l.share;
-                    const int wide = l.subs == 1 || l.per - from < kMaxVectors * V ? l.per - from : kMaxVectors * V;
-                    return (float)(left < l.share ? left : l.share) * (float)wide;
-                };
-                // four of a lane's pieces at a time, asked for together; up to 256 pieces are still there for the second sum
-                Moments m[4];
-                float c[4], sum = 0.0f, squares = 0.0f;
+            const Part p = part_of<S, V>(l, (int)a.c, (int)a.groups, slab);
+            // the first rows are on their way while the groups' moments are joined
+            const int64_t x_step = l.rows * a.x_p, z_step = SKIP ? l.rows * a.z_p : 0;
+            int64_t q = p.row < 0 ? end : begin + p.row;
+            const T* x = static_cast<const T*>(a.x) + i * a.x_n + (begin + p.row) * a.x_p + p.c;
+            const T* z = SKIP ? static_cast<const T*>(a.z) + i * a.z_n + (begin + p.row) * a.z_p + p.c : nullptr;
+            int here;
+            vec<T, V> held[R], skip[SKIP ? R : 1];
+            const auto load = [&]() {
+                here = end - q > (R - 1) * l.rows ? R : (int)(end - 1 - q) / l.rows + 1;
+                load_rows<S, T, R, V>(x, x_step, here, p, held);
+                x += R * x_step;
+                if constexpr (SKIP) {
+                    load_rows<S, T, R, V>(z, z_step, here, p, skip);
+                    z += R * z_step;
+                }
+            };
+            if (q < end) load();
+            float weight[V], bias[V], of_mean[V], scale[V];
+            load_affine<S, T, V>(a.weight, a.affine_type == DGNN_F32, p, 1.0f, weight);
+            load_affine<S, T, V>(a.bias, a.affine_type == DGNN_F32, p, 0.0f, bias);
+            // A wave joins two groups at once, so that what it waits for is asked for together; up to 256 pieces of each are still there for
+            // the second sum.  A lane behind the last piece reads that one and takes nothing of it.
+            for (int first = wave; first < p.groups; first += G * waves) {
+                const Moments* of[G];
+                Moments m[G][Q];
+                float mean[G] = {}, squares[G] = {};
+#pragma unroll
+                for (int k = 0; k < G; ++k) of[k] = moments + (i * a.groups + p.g0 + first + k * waves) * pieces;
+                const int groups = (p.groups - first + waves - 1) / waves;      // of this wave, from here on
                 const auto fetch = [&](int base) {
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const int piece = base + q * 64 + (threadIdx.x & 63);
-                        m[q] = piece < pieces ? of[piece] : Moments{0.0f, 0.0f};
-                        c[q] = piece < pieces ? count(piece) : 0.0f;
-                    }
+                    for (int q = 0; q < Q; ++q)
+                        if (base + q * 64 < pieces) {
+                            const int at = base + q * 64 + lane < pieces ? base + q * 64 + lane : pieces - 1;
+#pragma unroll
+                            for (int k = 0; k < G; ++k)
+                                if (k < groups) m[k][q] = of[k][at];
+                        }
                 };
-                for (int base = 0; base < pieces; base += 256) {
+                for (int base = 0; base < pieces; base += Q * 64) {
                     fetch(base);
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) sum = __builtin_fmaf(m[q].mean, c[q], sum);
-                }
-                const float mean = wave_sum(sum) * inverse;
-                for (int base = 0; base < pieces; base += 256) {
-                    if (pieces > 256) fetch(base);
+                    for (int q = 0; q < Q; ++q)
+                        if (base + q * 64 < pieces) {
+                            const bool is = base + q * 64 + lane < pieces;
+                            const float c = count(base + q * 64 + lane);
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const float d = m[q].mean - mean;
-                        squares += __builtin_fmaf(d * d, c[q], m[q].squares);
-                    }
+                            for (int k = 0; k < G; ++k)
+                                if (k < groups) mean[k] = is ? __builtin_fmaf(m[k][q].mean, c, mean[k]) : mean[k];
+                        }
                 }
-                squares = wave_sum(squares);
-                if ((threadIdx.x & 63) == 0) means[g] = mean, scales[g] = 1.0f / sqrtf(__builtin_fmaf(squares, inverse, a.eps));
+#pragma unroll
+                for (int k = 0; k < G; ++k)
+                    if (k < groups) mean[k] = wave_sum(mean[k]) * inverse;
+                for (int base = 0; base < pieces; base += Q * 64) {
+                    if (pieces > Q * 64) fetch(base);
+#pragma unroll
+                    for (int q = 0; q < Q; ++q)
+                        if (base + q * 64 < pieces) {
+                            const bool is = base + q * 64 + lane < pieces;
+                            const float c = count(base + q * 64 + lane);
+#pragma unroll
+                            for (int k = 0; k < G; ++k)
+                                if (k < groups) {
+                                    const float d = m[k][q].mean - mean[k];
+                                    squares[k] = is ? squares[k] + __builtin_fmaf(d * d, c, m[k][q].squares) : squares[k];
+                                }
+                        }
+                }
+#pragma unroll
+                for (int k = 0; k < G; ++k)
+                    if (k < groups) {
+                        const float all = wave_sum(squares[k]);
+                        if (lane == 0) means[first + k * waves] = mean[k], scales[first + k * waves] = 1.0f / sqrtf(__builtin_fmaf(all, inverse, a.eps));
+                    }
             }
             __syncthreads();
-            float weight[V], bias[V], mean[V], scale[V];
-            load_affine<T, V>(a.weight, a.affine_type == DGNN_F32, p, 1.0f, weight);
-            load_affine<T, V>(a.bias, a.affine_type == DGNN_F32, p, 0.0f, bias);
-            of_channels<V>(l, p, means, mean);
-            of_channels<V>(l, p, scales, scale);
+            of_channels<S, V>(l, p, means, of_mean);
+            of_channels<S, V>(l, p, scales, scale);
 #pragma unroll
             for (int e = 0; e < V; ++e) scale[e] *= weight[e];
             __syncthreads();                                    // (means and scales are the next slab's)
-            if (p.row < 0) continue;
-            for (int64_t q = begin + p.row; q < end; q += R * l.rows) {
-                const T* const x = static_cast<const T*>(a.x) + i * a.x_n + q * a.x_p + p.c;
-                T* y = static_cast<T*>(a.y) + i * a.y_n + q * a.y_p + p.c;
-                const int here = end - q > (R - 1) * l.rows ? R : (int)(end - 1 - q) / l.rows + 1;
-                vec<T, V> held[R], skip[SKIP ? R : 1];
-                load_rows<T, R, V, TINY>(x, l.rows * a.x_p, here, p, held);
-                if constexpr (SKIP) load_rows<T, R, V, TINY>(static_cast<const T*>(a.z) + i * a.z_n + q * a.z_p + p.c, l.rows * a.z_p, here, p, skip);
+            T* y = static_cast<T*>(a.y) + i * a.y_n + (begin + p.row) * a.y_p + p.c;
+            while (q < end) {
 #pragma unroll
                 for (int r = 0; r < R; ++r)
                     if (r < here) {
                         float v[V];
 #pragma unroll
                         for (int e = 0; e < V; ++e) {
-                            v[e] = __builtin_fmaf((float)held[r][e] - mean[e], scale[e], bias[e]);
+                            v[e] = __builtin_fmaf((float)held[r][e] - of_mean[e], scale[e], bias[e]);
                             if constexpr (SKIP) v[e] += (float)skip[r][e];
                         }
                         activate_kind<K>(v, a.activation);
-                        store_part<T, V>(y, p.n, v);
+                        store_part<S, T, V>(y, p.n, v);
                         y += l.rows * a.y_p;
                     }
+                q += R * l.rows;
+                if (q < end) load();
             }
         }
 }
@@ -462,11 +506,28 @@ int64_t groups_of_whole_lines(int64_t per, int64_t groups, int64_t vector)
     return line / per > 1 ? line / per : 1;
 }
 
+int vector_of(const dgnn_group_norm_args& a) { return a.type == DGNN_F32 ? 4 : 8; }
+
+Shape shape_of(const dgnn_group_norm_args& a, const Layout& l)
+{
+    const int vector = vector_of(a);
+    if (a.c < vector) return kTiny;
+    if (l.per % vector == 0) return kAligned;
+    return a.c % vector == 0 && l.per * l.groups_per_slab % vector == 0 && l.subs == 1 ? kWhole : kRagged;
+}
+
+// What group_sums needs: a number, or one for each channel, from every thread, or from every one of a wave's row.
+int scratch_of(const dgnn_group_norm_args& a, const Layout& l)
+{
+    const bool single = l.groups_per_slab == 1 || l.per % vector_of(a) == 0, even = (l.lanes & (l.lanes - 1)) == 0 && l.lanes <= 64;
+    return (even ? (l.threads + 63) / 64 * l.lanes : l.threads) * (single ? 1 : vector_of(a));
+}
+
 // One pass where a workgroup's registers hold a slab of a sample, two otherwise.
 Layout make_layout(const dgnn_group_norm_args& a, int* registers)
 {
     constexpr int kThreads = kMaxThreads / 2;                   // (1024 of four vectors hold what 512 of eight do)
-    const int vector = a.type == DGNN_F32 ? 4 : 8;
+    const int vector = vector_of(a);
     Layout l;
     l.per = (int)(a.c / a.groups);
     l.shares = 1;
@@ -480,56 +541,80 @@ Layout make_layout(const dgnn_group_norm_args& a, int* registers)
         l.lanes = (int)(subs > 1 ? kMaxVectors : ceil_div(groups * l.per, vector));
     };
     const auto held = [&]() { return (int64_t)(kThreads / l.lanes) * kRegisters; };
+    const auto may_halve = [&]() {
+        const int64_t now = groups * l.per, half = (groups + 1) / 2 * l.per;
+        return (half % vector == 0 || now % vector != 0) && (half >= 2 * vector || a.p <= 1024);
+    };
     cut(groups_of_whole_lines(l.per, a.groups, vector), 1);
     const int64_t whole = groups;
     *registers = 0;
-    // narrower slabs where these leave compute units idle, or do not fit and two vectors of a line would
-    while (groups > 1 && a.n * l.slabs < kUnitsWanted) cut((groups + 1) / 2, 1);
+    // Narrower slabs where these leave more than a quarter of the units idle, or do not fit and two vectors of a line would.  Not slabs whose rows
+    // end inside a vector where they do not yet (107 maps of 632 x 80, groups of ten: 16 us, 23 so), and single vectors of a line for short maps
+    // only: every workgroup fetches the whole line (2 maps of 4096 x 256: 18 us so, 12 in two passes; 114 of 1120 x 32: 11.4 us with two
+    // vectors for 228 workgroups, 18.6 with one for 456).
+    while (groups > 1 && a.n * l.slabs < kUnitsWanted * 3 / 4 && may_halve()) cut((groups + 1) / 2, 1);
     while (groups > 1 && groups * l.per > 2 * vector && a.p > held()) cut((groups + 1) / 2, 1);
     if (a.p <= held()) {
-        // as many vectors to a thread as give every unit 1024 of them: few where a call is one trip through the chip
+        // Eight vectors to a thread where the chip has about three or more for each of its threads (256 maps of 361 x 256: 32 us, 41 with four), two
+        // where a call is one trip through it (one map: 5.8, 6.7 with eight) -- unless the groups end inside vectors: what such a thread does
+        // beside its vectors is several times theirs (32 maps of 400 x 80, groups of ten: 8.7 us, 12 with two)
         const int64_t each_unit = a.n * l.slabs * l.lanes * a.p / (kUnitsWanted * kMaxThreads);
-        const int wanted = each_unit >= 6 ? kRegisters : each_unit >= 3 ? 4 : 2, most = wanted == kRegisters ? kThreads : kMaxThreads;
+        const int wanted = each_unit >= 3 || shape_of(a, l) == kWhole ? kRegisters : 2, most = wanted == kRegisters ? kThreads : kMaxThreads;
         l.threads = 64;
         while (l.threads < most && (l.threads < l.lanes || (int64_t)(l.threads / l.lanes) * wanted < a.p)) l.threads *= 2;
         l.rows = l.threads / l.lanes;
         const int64_t each = ceil_div(a.p, l.rows);
         *registers = each <= 2 ? 2 : each <= 4 ? 4 : 8;
+        l.scratch = scratch_of(a, l);
         return l;
     }
     const int subs = (int)ceil_div(l.per, kMaxVectors * vector);
     cut(subs > 1 ? 1 : whole, subs);
     l.threads = kThreads;
     l.rows = l.threads / l.lanes;
-    // shares enough for two workgroups on every unit
+    // shares enough for two workgroups on every unit; for one where that would leave a thread fewer rows than it loads at once, and mostly at work on
+    // what is the same for any number of rows
     int64_t shares = ceil_div(2 * kUnitsWanted, a.n * l.slabs);
+    if (shares * kRegisters * l.rows > a.p) shares = ceil_div(kUnitsWanted, a.n * l.slabs);
     if (shares > kMaxShares) shares = kMaxShares;
     l.share = ceil_div(ceil_div(a.p, shares), l.rows) * l.rows;
     l.shares = (int)ceil_div(a.p, l.share);
+    l.scratch = scratch_of(a, l);
     return l;
 }
 
-template <typename T, Kind K, bool SKIP, bool TINY>
-hipError_t launch_kind(const dgnn_group_norm_args& a, hipStream_t stream)
+template <Shape S, typename T, Kind K, bool SKIP>
+hipError_t launch_kind(const dgnn_group_norm_args& a, const Layout& l, int registers, hipStream_t stream)
 {
-    int registers;
-    const Layout l = make_layout(a, &registers);
     const dim3 grid((unsigned)(l.slabs < 65536 ? l.slabs : 65536), (unsigned)l.shares, (unsigned)(a.n < 32768 ? a.n : 32768)), block(l.threads);
-    if (registers == 2) return launch(one_pass_kernel<T, 2, K, SKIP, TINY>, grid, block, stream, a, l);
-    if (registers == 4) return launch(one_pass_kernel<T, 4, K, SKIP, TINY>, grid, block, stream, a, l);
-    if (registers == 8) return launch(one_pass_kernel<T, 8, K, SKIP, TINY>, grid, block, stream, a, l);
+    const size_t shared = 2 * (size_t)(l.scratch + l.groups_per_slab) * sizeof(float);
+    if (registers == 2) return launch_shared(one_pass_kernel<S, T, 2, K, SKIP>, grid, block, shared, stream, a, l);
+    if (registers == 4) return launch_shared(one_pass_kernel<S, T, 4, K, SKIP>, grid, block, shared, stream, a, l);
+    if (registers == 8) return launch_shared(one_pass_kernel<S, T, 8, K, SKIP>, grid, block, shared, stream, a, l);
     Moments* const moments = static_cast<Moments*>(a.workspace);
-    const hipError_t err = launch(moments_kernel<T, TINY>, grid, block, stream, a, l, moments);
-    return err != hipSuccess ? err : launch(apply_kernel<T, K, SKIP, TINY>, grid, block, stream, a, l, static_cast<const Moments*>(moments));
+    const hipError_t err = launch_shared(moments_kernel<S, T>, grid, block, shared, stream, a, l, moments);
+    return err != hipSuccess ? err : launch(apply_kernel<S, T, K, SKIP>, grid, block, stream, a, l, static_cast<const Moments*>(moments));
+}
+
+template <Shape S, typename T, bool SKIP>
+hipError_t launch_shape(const dgnn_group_norm_args& a, const Layout& l, int registers, hipStream_t stream)
+{
+    if (a.activation == DGNN_ACT_IDENTITY || a.activation == DGNN_ACT_RELU) return launch_kind<S, T, kPlain, SKIP>(a, l, registers, stream);
+    if (a.activation == DGNN_ACT_SILU) return launch_kind<S, T, kSilu, SKIP>(a, l, registers, stream);
+    return launch_kind<S, T, kAny, SKIP>(a, l, registers, stream);
 }
 
 template <typename T, bool SKIP>
 hipError_t launch_skip(const dgnn_group_norm_args& a, hipStream_t stream)
 {
-    if (a.c < width_of<T>) return launch_kind<T, kAny, SKIP, true>(a, stream);
-    if (a.activation == DGNN_ACT_IDENTITY || a.activation == DGNN_ACT_RELU) return launch_kind<T, kPlain, SKIP, false>(a, stream);
-    if (a.activation == DGNN_ACT_SILU) return launch_kind<T, kSilu, SKIP, false>(a, stream);
-    return launch_kind<T, kAny, SKIP, false>(a, stream);
+    int registers;
+    const Layout l = make_layout(a, &registers);
+    switch (shape_of(a, l)) {
+    case kAligned: return launch_shape<kAligned, T, SKIP>(a, l, registers, stream);
+    case kWhole: return launch_shape<kWhole, T, SKIP>(a, l, registers, stream);
+    case kRagged: return launch_kind<kRagged, T, kAny, SKIP>(a, l, registers, stream);
+    default: return launch_kind<kTiny, T, kAny, SKIP>(a, l, registers, stream);
+    }
 }
 
 template <typename T>
