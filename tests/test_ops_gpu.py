@@ -238,6 +238,20 @@ def test_group_norm_sizes(ops, shape, groups, dtype):
     group_norm_case(ops, shape, groups, t, "relu", affine=torch.float32, residual=True, shift=-3.0, seed=1)
 
 
+# where one way of cutting a call up ends and another begins: slabs that may be halved or not, short maps and long ones, one share and many, more
+# groups than the waves that join them, lines and vectors that groups end inside
+GN_CUTS = [((1, p, c), g) for p in (63, 64, 65, 1024, 1025, 2048, 2049, 4096, 4097) for c, g in ((64, 8), (80, 8), (96, 16))] + [
+    ((193, 9, 64), 8), ((191, 9, 64), 8), ((97, 33, 80), 8), ((3, 5241, 180), 9), ((1, 6193, 320), 32), ((2, 4500, 512), 512), ((2, 3000, 36), 9), ((7, 1515, 27), 9),
+    ((300, 15, 128), 16), ((2, 5000, 1100), 2), ((260, 513, 24), 3)]
+
+
+@pytest.mark.parametrize("shape,groups", GN_CUTS)
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_group_norm_where_the_cut_changes(ops, shape, groups, dtype):
+    t = TYPES[dtype]
+    group_norm_case(ops, shape, groups, t, "silu", affine=t, residual=True, seed=shape[1])
+
+
 @pytest.mark.parametrize("activation", ACTIVATIONS)
 @pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
 @pytest.mark.parametrize("shape,groups", [((3, 50, 40), 5), ((2, 361, 64), 8), ((1, 30000, 16), 2)])
