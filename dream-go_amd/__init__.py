@@ -5,6 +5,7 @@ the importable name ``dream_go_amd`` by ``__graft_entry__.package()`` / ``tests/
 
 Submodules
     api    ctypes mirror of the reference's ``dg_nn`` surface over the C ABI (include/dgnn.h)
+    ops    dense, group_norm and adjust_logits on device tensors (include/dgnn_ops.h)
     synth  synthetic networks / inputs in the reference's file formats
-    build  hipcc build of libdgnn_hip.so
+    build  hipcc build of libdgnn_hip.so and libdgnn_ops.so
 """
