@@ -57,7 +57,7 @@ typedef struct dgnn_dense_args {
     const void* bias;       /* [n] or NULL */
     const void* z;          /* [m][n] of out_type, row stride ldz (0: one row for all), or NULL; may be y itself */
     void* y;                /* [m][n] of out_type, row stride ldy; overlaps neither x nor w */
-    void* workspace;        /* dgnn_dense_workspace bytes, 256-byte aligned; NULL where that is 0 */
+    void* workspace;        /* dgnn_dense_workspace bytes, 256-byte aligned, apart from every operand; NULL where that is 0 */
     int64_t workspace_bytes;
     int64_t m, n, k;        /* 0 <= each < 2^31; k == 0: the sum is 0 */
     int64_t ldx, ldw, ldz, ldy;
@@ -82,7 +82,7 @@ typedef struct dgnn_group_norm_args {
     const void* bias;       /* [c] of affine_type, or NULL */
     const void* z;          /* [n][p][c] of `type`, strides z_n, z_p (0: repeated), or NULL */
     void* y;                /* [n][p][c] of `type`, strides y_n, y_p */
-    void* workspace;        /* dgnn_group_norm_workspace bytes, 256-byte aligned; NULL where that is 0 */
+    void* workspace;        /* dgnn_group_norm_workspace bytes, 256-byte aligned, apart from every operand; NULL where that is 0 */
     int64_t workspace_bytes;
     int64_t n, p, c, groups;
     int64_t x_n, x_p, z_n, z_p, y_n, y_p;

@@ -242,7 +242,7 @@ def test_group_norm_sizes(ops, shape, groups, dtype):
 # groups than the waves that join them, lines and vectors that groups end inside
 GN_CUTS = [((1, p, c), g) for p in (63, 64, 65, 1024, 1025, 2048, 2049, 4096, 4097) for c, g in ((64, 8), (80, 8), (96, 16))] + [
     ((193, 9, 64), 8), ((191, 9, 64), 8), ((97, 33, 80), 8), ((3, 5241, 180), 9), ((1, 6193, 320), 32), ((2, 4500, 512), 512), ((2, 3000, 36), 9), ((7, 1515, 27), 9),
-    ((300, 15, 128), 16), ((2, 5000, 1100), 2), ((260, 513, 24), 3)]
+    ((300, 15, 128), 16), ((2, 5000, 1100), 2), ((260, 513, 24), 3), ((64, 361, 90), 9), ((193, 700, 20), 2)]
 
 
 @pytest.mark.parametrize("shape,groups", GN_CUTS)
