@@ -1,12 +1,13 @@
 // dgnn_group_norm: group norm over channels-last maps, the skip input and the activation applied on the way out.
 //
 // A workgroup owns a slab of channels of one sample -- whole groups, up to 64 sixteen-byte vectors -- and all positions, or a share of them.
-// Threads are laid over (position, vector), so that neighbours read what lies side by side.  Mean and variance take two passes over values that
-// are in REGISTERS: the variance is the mean of squared differences from the mean, never a difference of sums, and costs no second read.
+// Threads are laid over (position, vector), so that neighbours read what lies side by side.
 //
-//   one pass   a sample's slab fits the registers of a workgroup: read once, written once, which is the floor
-//   two        it does not: a first kernel leaves (mean, sum of squares about it) of every share of the positions, a second joins those of its
-//              groups -- about their joint mean, in a fixed order -- and reads the maps again, mostly out of the last-level cache
+//   one pass   a sample's slab fits the registers of a workgroup: read once, written once, which is the floor.  Mean and variance are two passes over
+//              values that are in registers: the variance is the mean of squared differences from the mean and costs no second read
+//   two        it does not: a first kernel leaves (mean, sum of squares about it) of every share of the positions, gathered eight rows at a time
+//              about the mean of the rows before (moments_kernel says what that loses); a second joins those of its groups -- about their joint
+//              mean, in a fixed order -- and reads the maps again, mostly out of the last-level cache
 //
 // Large maps are bound by memory on both ways; the activations are branch-free for that reason (ops_device.h).  256 maps of 361 x 256 fp16 with a
 // skip (142 MB) take 32.5 us in one pass, 4.4 TB/s; 8 maps of 16384 x 320 bf16 with SiLU (168 MB, its input read twice) 58 us in two, 2.9 TB/s
@@ -22,7 +23,8 @@ namespace {
 
 constexpr int kMaxThreads = 1024, kMaxVectors = 64, kRegisters = 8;     // vectors of a row of a slab; vectors of a thread
 constexpr int kMaxGroups = kMaxVectors * 8;                             // of a slab
-constexpr int kMaxShares = 256;                                         // of a sample's positions
+constexpr int kMaxShares = 256;                                         // of a sample's positions, where these are not more than
+constexpr int kSerialRows = 2048;                                       // a thread adds up one after the other
 constexpr int kUnitsWanted = 256;                                       // workgroups that give every compute unit one
 
 template <typename T> constexpr int width_of = 16 / (int)sizeof(T);     // elements of a vector
@@ -301,10 +303,14 @@ struct Moments {
 
 // (mean, squares) of a share of the positions of a slab's groups, to moments[sample][group][share][sub].
 //
-// Each thread sums, channel by channel, the differences of its rows from its FIRST row and their squares: four operations a value, where a second
-// look at the values would take six, and this kernel is bound by them as much as by memory.  The shift is one of the n values it is taken from, so
-// n (mean - shift)^2 is less than n times the sum of squares about the mean, whatever the values are: n times a rounding is all that the
-// difference `square - sum^2 / n` can lose.  The threads of a group are then joined about their common mean.
+// Each thread takes its rows by eights and sums, channel by channel, their differences from the mean of the rows BEFORE them (the first eight: from
+// its first row) and the squares of those: four operations a value, where a second look at the values would take six, and this kernel is bound by them
+// as much as by memory.  With s and q the two sums, m the mean of n - 8 rows and n those with the eight, the rows join as
+//   mean = m + s / n,   squares about it += q - s^2 / n,
+// in which s^2 / n is at most half of q (s^2 <= 8 q, n >= 16): a difference that loses one bit at most, whatever the rows are.  For the first eight
+// the shift is one of the values themselves, 8 (mean - shift)^2 is at most eight times the sum of squares about the mean, and the difference loses
+// a few.  No sum runs over more than kSerialRows / 8 joins (make_layout), each of them a few half steps of fp32.  The threads of a group are then
+// joined about their common mean.
 template <Shape S, typename T>
 __global__ __launch_bounds__(kMaxThreads / 2, 4)
 void moments_kernel(dgnn_group_norm_args a, Layout l, Moments* moments)
@@ -319,7 +325,7 @@ void moments_kernel(dgnn_group_norm_args a, Layout l, Moments* moments)
             const Part p = part_of<S, V>(l, (int)a.c, (int)a.groups, slab);
             const float inverse = 1.0f / ((float)(end - begin) * (float)(l.subs > 1 ? p.channels : l.per));
             const int rows = (int)(end - begin), here = p.row < 0 || p.row >= rows ? 0 : (rows - 1 - p.row) / l.rows + 1;
-            float shift[V] = {}, sum[V] = {}, square[V] = {};
+            float mean[V] = {}, squared[V] = {};
             if (here > 0) {
                 const int64_t step = l.rows * a.x_p;
                 const T* x = static_cast<const T*>(a.x) + i * a.x_n + (begin + p.row) * a.x_p + p.c;
@@ -330,36 +336,38 @@ void moments_kernel(dgnn_group_norm_args a, Layout l, Moments* moments)
                     x += R * step;
                     if (done == 0) {
 #pragma unroll
-                        for (int e = 0; e < V; ++e) shift[e] = (float)held[0][e];
+                        for (int e = 0; e < V; ++e) mean[e] = (float)held[0][e];
                     }
+                    float sum[V] = {}, square[V] = {};
 #pragma unroll
                     for (int r = 0; r < R; ++r)
                         if (r < now) {
 #pragma unroll
                             for (int e = 0; e < V; ++e) {
-                                const float d = (float)held[r][e] - shift[e];
+                                const float d = (float)held[r][e] - mean[e];
                                 sum[e] += d;
                                 square[e] = __builtin_fmaf(d, d, square[e]);
                             }
                         }
+                    const float each = rcp((float)(done + now));
+#pragma unroll
+                    for (int e = 0; e < V; ++e) {
+                        const float moved = sum[e] * each, more = __builtin_fmaf(-moved, sum[e], square[e]);
+                        mean[e] += moved;
+                        squared[e] += more < 0.0f ? 0.0f : more;       // (a NaN stays)
+                    }
                 }
             }
-            const float count = (float)here, each = here > 0 ? 1.0f / count : 0.0f;
-            float mean[V], mine[V], joint[V];
+            const float count = (float)here;
+            float mine[V], joint[V];
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const float about = sum[e] * each;
-                square[e] = __builtin_fmaf(-about, sum[e], square[e]);
-                square[e] = square[e] < 0.0f ? 0.0f : square[e];       // (a NaN stays)
-                mean[e] = shift[e] + about;
-                mine[e] = e < p.n ? mean[e] * count : 0.0f;
-            }
+            for (int e = 0; e < V; ++e) mine[e] = e < p.n ? mean[e] * count : 0.0f;
             group_sums<S, V>(l, p, mine, scratch, means, [&](float s) { return s * inverse; });
             of_channels<S, V>(l, p, means, joint);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 const float d = mean[e] - joint[e];
-                mine[e] = e < p.n ? __builtin_fmaf(d * d, count, square[e]) : 0.0f;
+                mine[e] = e < p.n ? __builtin_fmaf(d * d, count, squared[e]) : 0.0f;
             }
             group_sums<S, V>(l, p, mine, scratch + l.scratch, squares, [&](float s) { return s; });
             for (int g = threadIdx.x; g < p.groups; g += blockDim.x)
@@ -577,6 +585,9 @@ Layout make_layout(const dgnn_group_norm_args& a, int* registers)
     int64_t shares = ceil_div(2 * kUnitsWanted, a.n * l.slabs);
     if (shares * kRegisters * l.rows > a.p) shares = ceil_div(kUnitsWanted, a.n * l.slabs);
     if (shares > kMaxShares) shares = kMaxShares;
+    // and as many as keep a thread's rows few.  (At most 2^37 elements a sample: fewer than 40000, whatever the lanes)
+    const int64_t least = ceil_div(a.p, (int64_t)kSerialRows * l.rows);
+    if (shares < least) shares = least;
     l.share = ceil_div(ceil_div(a.p, shares), l.rows) * l.rows;
     l.shares = (int)ceil_div(a.p, l.share);
     l.scratch = scratch_of(a, l);

@@ -1,0 +1,56 @@
+"""Where the operators of dream_go_amd.ops could lose digits that their formulas keep, against 64 bits, on a GPU.
+
+Every tolerance counts half steps of fp32 (ULP) along the longest run of roundings that the form under test has, and the one rounding of the result."""
+import math
+
+import pytest
+
+from test_ops_gpu import TYPES, ULP, gen
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+
+@pytest.fixture(scope="module")
+def ops(api):
+    from dream_go_amd import ops as module
+    return module
+
+
+# ---- group norm ---------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("n,p,c,groups,dtype", [(512, 65536, 64, 8, "fp16"), (512, 32768, 64, 8, "fp32"), (1, 1 << 24, 64, 32, "bf16")])
+def test_group_norm_of_flat_maps_behind_a_border(ops, n, p, c, groups, dtype):
+    """The first rows lie far from all others, which are equal, and a thread adds up a thousand of them: what each of them adds to the variance is
+    rounded the same way every time.  The moments are joined eight rows at a time, at most 2048 / 8 = 256 joins, each within a few half steps."""
+    x = torch.full((n, p, c), 0.123, dtype=TYPES[dtype], device="cuda")
+    border, edge, flat = 64, 1000.0, float(x[0, 0, 0])
+    x[:, :border] = edge
+    y = ops.group_norm(x, groups, eps=0.0)
+    f = border / p
+    mean, sd = f * edge + (1 - f) * flat, (edge - flat) * math.sqrt(f * (1 - f))
+    for part, value in ((y[:, :border], edge), (y[:, border:], flat)):
+        want = (value - mean) / sd
+        slack = 512 * ULP * (abs(want) + (abs(value) + abs(mean)) / sd)
+        bound = torch.finfo(y.dtype).eps / 2 * (abs(want) + slack) + slack
+        low, high = float(part.min()), float(part.max())
+        assert abs(low - want) <= bound and abs(high - want) <= bound, (value, low, high, want, bound)
+
+
+@pytest.mark.parametrize("shape,groups", [((2, 361, 64), 8), ((3, 7, 30), 3), ((1, 1000, 90), 9), ((1, 50000, 16), 4), ((2, 20000, 40), 4)])
+def test_group_norm_keeps_the_variance_of_values_far_from_zero(ops, shape, groups):
+    """A mean fifteen hundred away: squares of values differ in their last bits only.  No thread here adds up more than 8 rows of 8 values one after the
+    other, trees join the rest: 96 half steps are more than either form has."""
+    serial = 96
+    n, p, c = shape
+    x = (torch.randn(shape, generator=gen(3)) + 1500.0).float()
+    v = x.double().reshape(n, p, groups, c // groups)
+    d = v - v.mean((1, 3), keepdim=True)
+    var = (d * d).mean((1, 3), keepdim=True)
+    y = ops.group_norm(x.cuda(), groups, eps=0.0).cpu()
+    off = serial * ULP * 1500.0 / var.sqrt()                                   # of the mean, in standard deviations
+    got = y.double().reshape(v.shape)
+    assert ((got - d / var.sqrt()).abs() <= off + (serial * ULP + off * off) * (d / var.sqrt()).abs()).all()
+    spread = got.var((1, 3), unbiased=False)
+    assert ((spread - 1).abs() <= 2 * serial * ULP + (off * off).reshape(spread.shape)).all(), spread

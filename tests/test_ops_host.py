@@ -153,3 +153,15 @@ def test_tensors_of_the_cpu_are_refused(ops, api):
         with pytest.raises(api.Error) as e:
             run()
         assert e.value.status == api.BAD_ARGUMENT
+
+
+@pytest.mark.parametrize("n", [1, 512])
+@pytest.mark.parametrize("p,c,lanes,type_", [((1 << 31) - 1, 8, 1, F16), (1 << 28, 64, 8, BF16), ((1 << 29) - 64, 256, 64, F32), (1 << 20, 320, None, F16)])
+def test_no_thread_adds_up_more_rows_than_the_sums_are_good_for(ops, n, p, c, lanes, type_):
+    """A workspace holds eight bytes for every share of the positions; a share's rows are dealt to 512 threads, `lanes` of them side by side."""
+    args = dict(GROUP_NORM, n=n, p=p, c=c, groups=1 if lanes else 32, x_n=p * c, x_p=c, y_n=p * c, y_p=c, z=0, x=1 << 50, y=1 << 54, type=type_, affine_type=F32)
+    need = ctypes.c_int64()
+    assert ops.lib.dgnn_group_norm_workspace(ops._GROUP_NORM.pack(*args.values()), need) == OK
+    shares = need.value // (8 * n * args["groups"])
+    assert 0 < shares <= 65535                                                # a grid's second extent
+    assert -(-p // shares) <= 2048 * (512 // (lanes or 64 // 4))
