@@ -367,7 +367,7 @@ void moments_kernel(dgnn_group_norm_args a, Layout l, Moments* moments)
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 const float d = mean[e] - joint[e];
-                mine[e] = e < p.n ? __builtin_fmaf(d * d, count, squared[e]) : 0.0f;
+                mine[e] = e < p.n && here > 0 ? __builtin_fmaf(d * d, count, squared[e]) : 0.0f;      // (no row: d * d may be infinite, times 0 no number)
             }
             group_sums<S, V>(l, p, mine, scratch + l.scratch, squares, [&](float s) { return s; });
             for (int g = threadIdx.x; g < p.groups; g += blockDim.x)

@@ -5,7 +5,7 @@ import math
 
 import pytest
 
-from test_ops_gpu import TYPES, ULP, gen
+from test_ops_gpu import TYPES, ULP, close, gen, group_norm64
 
 pytestmark = pytest.mark.gpu
 
@@ -36,6 +36,21 @@ def test_group_norm_of_flat_maps_behind_a_border(ops, n, p, c, groups, dtype):
         bound = torch.finfo(y.dtype).eps / 2 * (abs(want) + slack) + slack
         low, high = float(part.min()), float(part.max())
         assert abs(low - want) <= bound and abs(high - want) <= bound, (value, low, high, want, bound)
+
+
+@pytest.mark.parametrize("shape,groups", [((1, 40000, 64), 8), ((2, 33333, 24), 3), ((1, 70001, 8), 1)])
+def test_group_norm_of_huge_values_that_differ_little(ops, shape, groups):
+    """Around 2^70 the square of a value is no number of fp32 any more; differences from the mean of at most 2^56 have squares of which half a million add
+    up to less than 2^128.  The last share of the positions has threads without a row."""
+    step = torch.finfo(torch.float32).eps * 2.0 ** 70
+    x = (2.0 ** 70 + step * torch.randint(0, 500, shape, generator=gen(5)).double()).float()
+    pre, _ = group_norm64(x, groups, None, None, None, 0.0)
+    n, p, c = shape
+    v = x.double().reshape(n, p, groups, c // groups)
+    scale = (1 / v.std((1, 3), unbiased=False, keepdim=True)).expand_as(v).reshape(shape)
+    # the mean is off by 64 half steps of its size at most, the variance by the square of that beside itself
+    off = 64 * ULP * 2.0 ** 70 * scale
+    close(ops.group_norm(x.cuda(), groups, eps=0.0), pre, off + (64 * ULP + off * off) * pre.abs(), (shape, groups))
 
 
 @pytest.mark.parametrize("shape,groups", [((2, 361, 64), 8), ((3, 7, 30), 3), ((1, 1000, 90), 9), ((1, 50000, 16), 4), ((2, 20000, 40), 4)])
