@@ -30,6 +30,9 @@ hipError_t launch(void (*kernel)(Params...), dim3 grid, dim3 block, hipStream_t 
 // A grid dimension times the workgroup's has to stay below 2^32; kernels loop over what a capped grid leaves.
 constexpr int64_t kMaxGrid = 1 << 20;
 
+// How far a vector of `width` channels from channel c on reaches beyond the last of them.  (c + width may be more than 32 bits hold.)
+__host__ __device__ constexpr int overhang(int c, int width, int channels) { return c > channels - width ? c - (channels - width) : 0; }
+
 int64_t dense_workspace(const dgnn_dense_args& a);
 hipError_t launch_dense(const dgnn_dense_args& a, hipStream_t stream);
 int64_t group_norm_workspace(const dgnn_group_norm_args& a);

@@ -75,11 +75,11 @@ __device__ __forceinline__ Part part_of(const Layout& l, int channels, int group
         c0 = p.g0 * l.per + first;
     }
     p.at = lane * V;
-    p.c = c0 + p.at;
     p.n = p.channels - p.at < V ? p.channels - p.at : V;
     p.row = row < l.rows && p.n > 0 ? row : -1;
-    if (p.row < 0) p.at = p.n = 0, p.c = c0;
-    p.back = S <= kWhole || p.c + V <= channels ? 0 : p.c + V - channels;
+    if (p.row < 0) p.at = p.n = 0;
+    p.c = c0 + p.at;
+    p.back = S <= kWhole ? 0 : overhang(p.c, V, channels);
     return p;
 }
 

@@ -69,3 +69,22 @@ def test_group_norm_keeps_the_variance_of_values_far_from_zero(ops, shape, group
     assert ((got - d / var.sqrt()).abs() <= off + (serial * ULP + off * off) * (d / var.sqrt()).abs()).all()
     spread = got.var((1, 3), unbiased=False)
     assert ((spread - 1).abs() <= 2 * serial * ULP + (off * off).reshape(spread.shape)).all(), spread
+
+
+def test_group_norm_of_nearly_two_to_the_31_channels(ops):
+    """The last vector of a row begins eight channels in front of 2^31 and ends inside it."""
+    c, pad = 2147483646, 16
+    buffer = torch.empty(c + pad, dtype=torch.bfloat16, device="cuda").normal_(generator=torch.Generator(device="cuda").manual_seed(1))
+    buffer[c:] = math.nan
+    x, bias = buffer[:c].view(1, 1, c), torch.empty(c, dtype=torch.bfloat16, device="cuda").fill_(0.5)
+    out = torch.full((c + pad,), 3.0, dtype=torch.bfloat16, device="cuda")
+    y = out[:c].view(1, 1, c)
+    assert ops.group_norm(x, c // 2, None, bias, out=y) is y
+    for begin in (0, (1 << 30) - 4, c - (1 << 20)):                            # pairs of channels: each is half their difference from the mean
+        pair = x[0, 0, begin:begin + (1 << 20)].double().view(-1, 2)
+        d = (pair - pair.mean(1, keepdim=True))
+        want = (d / torch.sqrt((d * d).mean(1, keepdim=True) + 1e-5) + 0.5).flatten()
+        got = y[0, 0, begin:begin + (1 << 20)].double()
+        slack = 32 * ULP * (1 + want.abs())
+        assert ((got - want).abs() <= 2.0 ** -8 * (want.abs() + slack) + slack).all()
+    assert not y.isnan().any() and (out[c:] == 3.0).all()

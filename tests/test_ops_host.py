@@ -165,3 +165,13 @@ def test_no_thread_adds_up_more_rows_than_the_sums_are_good_for(ops, n, p, c, la
     shares = need.value // (8 * n * args["groups"])
     assert 0 < shares <= 65535                                                # a grid's second extent
     assert -(-p // shares) <= 2048 * (512 // (lanes or 64 // 4))
+
+
+def test_channels_are_counted_without_overflow(tmp_path):
+    """Up to 2^31 - 1 channels.  An overflow is no constant expression: the compiler refuses it."""
+    cases = [(0, 8, 8, 0), (0, 8, 5, 3), (8, 8, 13, 3), (8, 8, 16, 0), (0, 4, 1, 3), (2147483640, 8, 2147483647, 1), (2147483640, 8, 2147483646, 2),
+             (2147483632, 8, 2147483647, 0), (2147483646, 1, 2147483647, 0), (2147483644, 4, 2147483647, 1)]
+    lines = "".join(f"static_assert(dgnn::ops::overhang({c}, {width}, {channels}) == {want});\n" for c, width, channels, want in cases)
+    (tmp_path / "s.cpp").write_text('#include "ops.h"\n' + lines)
+    subprocess.run(["g++", "-std=c++17", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include", "-I", os.path.join(ROOT, "dream-go_amd", "csrc"), "-fsyntax-only", str(tmp_path / "s.cpp")],
+                   check=True)
