@@ -9,7 +9,8 @@ namespace dgnn {
 namespace ops {
 
 // Launches `kernel` and returns what the launch itself said (hipGetLastError would also return, and clear, what others left there).
-// `shared`: bytes of LDS beyond what the kernel declares, 64 KiB at most.
+// `shared`: bytes of LDS beyond what the kernel declares; both together kMaxShared at most (each caller asserts its own bound).
+constexpr size_t kMaxShared = 160 * 1024;
 template <typename... Params>
 hipError_t launch_as(void (*kernel)(Params...), dim3 grid, dim3 block, size_t shared, hipStream_t stream, Params... args)
 {

@@ -598,6 +598,8 @@ template <Shape S, typename T, Kind K, bool SKIP>
 hipError_t launch_kind(const dgnn_group_norm_args& a, const Layout& l, int registers, hipStream_t stream)
 {
     const dim3 grid((unsigned)(l.slabs < 65536 ? l.slabs : 65536), (unsigned)l.shares, (unsigned)(a.n < 32768 ? a.n : 32768)), block(l.threads);
+    // (up to 66048 bytes: 1024 threads with a number for each of eight channels, twice, where 64 groups end inside vectors)
+    static_assert(2 * (kMaxThreads * 8 + kMaxGroups) * sizeof(float) <= kMaxShared, "what a compute unit has");
     const size_t shared = 2 * (size_t)(l.scratch + l.groups_per_slab) * sizeof(float);
     if (registers == 2) return launch_shared(one_pass_kernel<S, T, 2, K, SKIP>, grid, block, shared, stream, a, l);
     if (registers == 4) return launch_shared(one_pass_kernel<S, T, 4, K, SKIP>, grid, block, shared, stream, a, l);

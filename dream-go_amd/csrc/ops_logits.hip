@@ -171,6 +171,7 @@ hipError_t launch_typed(const dgnn_logits_args& a, hipStream_t stream)
     const int chunks = (int)((a.v + chunk - 1) / chunk);
     const dim3 grid((unsigned)(chunks < (1 << 20) ? chunks : 1 << 20), (unsigned)(a.b < 65535 ? a.b : 65535));
     if (!history) return launch(logits_kernel<T, O, int32_t, false, false>, grid, dim3(threads), stream, a, chunk, chunks);
+    static_assert(kMaxChunk * sizeof(unsigned) <= kMaxShared / 2, "two workgroups on a unit");
     const size_t shared = chunk * sizeof(unsigned);
     const bool wide = a.history_type == DGNN_I64, many = a.t >= kLongHistory;
     if (many && wide) return launch_shared(logits_kernel<T, O, int64_t, true, true>, grid, dim3(threads), shared, stream, a, chunk, chunks);

@@ -5,7 +5,7 @@ import math
 
 import pytest
 
-from test_ops_gpu import TYPES, ULP, close, gen, group_norm64
+from test_ops_gpu import TYPES, ULP, close, gen, group_norm64, group_norm_case
 
 pytestmark = pytest.mark.gpu
 
@@ -88,3 +88,10 @@ def test_group_norm_of_nearly_two_to_the_31_channels(ops):
         slack = 32 * ULP * (1 + want.abs())
         assert ((got - want).abs() <= 2.0 ** -8 * (want.abs() + slack) + slack).all()
     assert not y.isnan().any() and (out[c:] == 3.0).all()
+
+
+@pytest.mark.parametrize("shape,groups", [((96, 43, 195), 65), ((192, 43, 189), 63), ((96, 72, 455), 65)])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_group_norm_with_all_the_lds_it_may_ask_for(ops, shape, groups, dtype):
+    """1024 threads with one number for each of eight channels: 66048 bytes are the most that a call asks for."""
+    group_norm_case(ops, shape, groups, TYPES[dtype], "relu", affine=TYPES[dtype], residual=True, seed=groups)
