@@ -80,7 +80,8 @@ void logits_kernel(dgnn_logits_args, int chunk, int chunks)
             };
             fetch(0);
 
-            float repetition = 1.0f, inverse = 1.0f, presence = 0.0f, frequency = 0.0f;
+            float repetition = 1.0f, mantissa = 1.0f, inverse = 1.0f, presence = 0.0f, frequency = 0.0f;     // repetition: mantissa 2^-exponent
+            int exponent = 0;
             if constexpr (HISTORY) {
                 const Arguments a = again(args);
                 const int t = (int)a->t, wanted = a->lengths ? a->lengths[i] : t, given = a->prompt_lengths ? a->prompt_lengths[i] : 0;
@@ -109,13 +110,23 @@ void logits_kernel(dgnn_logits_args, int chunk, int chunks)
                 __syncthreads();
                 const Arguments p = again(args);
                 repetition = p->repetition ? p->repetition[i] : p->repetition_all;
-                inverse = 1.0f / repetition;
+                mantissa = 2.0f * __builtin_amdgcn_frexp_mantf(repetition);
+                exponent = 1 - __builtin_amdgcn_frexp_expf(repetition);
+                inverse = 1.0f / mantissa;
                 presence = p->presence ? p->presence[i] : p->presence_all;
                 frequency = p->frequency ? p->frequency[i] : p->frequency_all;
             }
+            // l / repetition to the last bit: a quotient by the reciprocal, corrected by what the exact product with it leaves of l (fixup: where l is
+            // infinite).  By a mantissa, so that the reciprocal is no matter of range.  256 rows of 131072 with it 40.3 us, with the compiler's division 42.8,
+            // with the product alone, which is a step off now and then, 39.4.
+            const auto divided = [&](float l) {
+                float q = l * inverse;
+                q = __builtin_fmaf(__builtin_fmaf(-q, mantissa, l), inverse, q);
+                return __builtin_ldexpf(__builtin_amdgcn_div_fixupf(q, mantissa, l), exponent);
+            };
             const auto penalize = [&](float l, unsigned count) {
                 const unsigned answered = count & kAnswers<LONG>;
-                const float p = l * (l > 0.0f ? inverse : repetition) - frequency * (float)answered;
+                const float p = (l > 0.0f ? divided(l) : l * repetition) - frequency * (float)answered;
                 return count ? p - (answered ? presence : 0.0f) : l;
             };
             for (int base = 0; base < n; base += kEach * 8 * blockDim.x) {

@@ -95,3 +95,21 @@ def test_group_norm_of_nearly_two_to_the_31_channels(ops):
 def test_group_norm_with_all_the_lds_it_may_ask_for(ops, shape, groups, dtype):
     """1024 threads with one number for each of eight channels: 66048 bytes are the most that a call asks for."""
     group_norm_case(ops, shape, groups, TYPES[dtype], "relu", affine=TYPES[dtype], residual=True, seed=groups)
+
+
+# ---- logits -----------------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("b,v", [(3, 362), (5, 20011)])
+def test_a_repetition_divides(ops, b, v):
+    """One rounding, that of l / repetition or l * repetition: the bits are those of the one operation."""
+    g = gen(8)
+    logits = torch.randn(b, v, generator=g) * 5
+    history = torch.arange(v, dtype=torch.int32).expand(b, v).contiguous()
+    r = torch.rand(b, generator=g) + 0.7
+    want = torch.where(logits > 0, logits / r[:, None], logits * r[:, None])
+    assert torch.equal(ops.adjust_logits(logits.cuda(), history=history.cuda(), repetition=r.cuda()).cpu(), want)
+    # where 1 / repetition is no number of fp32, l / repetition may be one
+    tiny = torch.full((b,), 2.0 ** -130)
+    small = logits * 2.0 ** -100
+    got = ops.adjust_logits(small.cuda(), history=history.cuda(), repetition=tiny.cuda()).cpu()
+    assert torch.equal(got[small > 0], (small / tiny[:, None])[small > 0])
