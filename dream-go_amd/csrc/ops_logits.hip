@@ -4,7 +4,7 @@
 // history into LDS -- the tokens of its chunk only, by integer atomics, whose order does not show -- and then adjusts and writes what it
 // has.  Memory bounds it as long as a history is short beside the vocabulary: every chunk reads the whole history (out of the L2), so chunks are as
 // large as LDS allows two of on a compute unit, and smaller only where that leaves units idle.  256 rows of 131072 bf16 logits with 8192 tokens of
-// history each: 38.5 us, 3.8 TB/s; 32 of 50257 fp32: 7.3 us; one of 362: 4.8, of which a launch is 2.5.
+// history each: 40.3 us, 3.65 TB/s; 32 of 50257 fp32: 7.25 us; one of 362: 4.8, of which a launch is 2.5.
 #include "ops_device.h"
 
 namespace dgnn {
@@ -12,7 +12,8 @@ namespace ops {
 namespace {
 
 constexpr int kMaxChunk = 16384, kMinChunk = 1024;      // tokens; 4 bytes of LDS each
-constexpr int kEach = 2;                                // vectors of eight tokens that a thread holds at a time
+constexpr int kMaxThreads = 1024, kEach = 2;            // vectors of eight tokens that a thread holds
+static_assert(kMaxThreads * kEach * 8 >= kMaxChunk, "a workgroup holds its chunk");
 
 // What is counted of a token: how often it occurs in the given part, above, and in the answer part, below.  A history of fewer than 65536 tokens
 // fits sixteen bits each, and one kind of atomic does; with LONG one bit says that the given part has it at all.
@@ -53,7 +54,7 @@ struct Chunk {
 
 // HISTORY: H is the type of its tokens.
 template <typename T, typename O, typename H, bool HISTORY, bool LONG>
-__global__ __launch_bounds__(1024, 8)                   // two workgroups on a unit: one counts while the other writes
+__global__ __launch_bounds__(kMaxThreads, 8)            // two workgroups on a unit: one counts while the other writes
 void logits_kernel(dgnn_logits_args, int chunk, int chunks)
 {
     const Arguments args = (Arguments)__builtin_amdgcn_kernarg_segment_ptr();   // (the first parameter)
@@ -65,11 +66,11 @@ void logits_kernel(dgnn_logits_args, int chunk, int chunks)
             const int n = left < chunk ? (int)left : chunk;
             vec<T, 8> held[kEach];
             unsigned allowed[kEach];
-            const auto fetch = [&](int base) {
+            {
                 const Chunk<T, O> at(again(args), i, v0);
 #pragma unroll
                 for (int q = 0; q < kEach; ++q) {
-                    const int e = base + (q * (int)blockDim.x + (int)threadIdx.x) * 8;
+                    const int e = (q * (int)blockDim.x + (int)threadIdx.x) * 8;
                     held[q] = vec<T, 8>{};
                     allowed[q] = 0xff;
                     if (e + 8 <= n) {
@@ -77,8 +78,7 @@ void logits_kernel(dgnn_logits_args, int chunk, int chunks)
                         if (at.mask) allowed[q] = at.mask[e >> 3];
                     }
                 }
-            };
-            fetch(0);
+            }
 
             float repetition = 1.0f, mantissa = 1.0f, inverse = 1.0f, presence = 0.0f, frequency = 0.0f;     // repetition: mantissa 2^-exponent
             int exponent = 0;
@@ -129,36 +129,33 @@ void logits_kernel(dgnn_logits_args, int chunk, int chunks)
                 const float p = (l > 0.0f ? divided(l) : l * repetition) - frequency * (float)answered;
                 return count ? p - (answered ? presence : 0.0f) : l;
             };
-            for (int base = 0; base < n; base += kEach * 8 * blockDim.x) {
-                if (base > 0) fetch(base);
-                const Chunk<T, O> at(again(args), i, v0);
+            const Chunk<T, O> at(again(args), i, v0);
 #pragma unroll
-                for (int q = 0; q < kEach; ++q) {
-                    const int e = base + (q * (int)blockDim.x + (int)threadIdx.x) * 8;
-                    if (e + 8 <= n) {
-                        vec<float, 8> l = __builtin_convertvector(held[q], vec<float, 8>);
-                        if constexpr (HISTORY) {
-                            const vec<unsigned, 8> counts = *reinterpret_cast<const vec<unsigned, 8>*>(seen + e);
+            for (int q = 0; q < kEach; ++q) {
+                const int e = (q * (int)blockDim.x + (int)threadIdx.x) * 8;
+                if (e + 8 <= n) {
+                    vec<float, 8> l = __builtin_convertvector(held[q], vec<float, 8>);
+                    if constexpr (HISTORY) {
+                        const vec<unsigned, 8> counts = *reinterpret_cast<const vec<unsigned, 8>*>(seen + e);
 #pragma unroll
-                            for (int r = 0; r < 8; ++r)
-                                if (__builtin_amdgcn_ballot_w64(counts[r] != 0)) l[r] = penalize(l[r], counts[r]);      // (most of a vocabulary is never seen)
-                        }
-                        if (at.bias) l += at.bias_is_float ? load_eight(reinterpret_cast<const float*>(at.bias) + e) : load_eight(reinterpret_cast<const T*>(at.bias) + e);
-                        if (at.mask) {
-#pragma unroll
-                            for (int r = 0; r < 8; ++r) l[r] = allowed[q] & 1u << r ? l[r] : -INFINITY;
-                        }
-                        store_vec<O, 8>(at.out + e, __builtin_convertvector(l, vec<O, 8>));
-                    } else {
-                        for (int r = e; r < n; ++r) {
-                            float l = (float)at.logits[r];
-                            if constexpr (HISTORY) l = penalize(l, seen[r]);
-                            if (at.bias) l += load_either<T>(at.bias, r, at.bias_is_float);
-                            at.out[r] = (O)(!at.mask || (at.mask[r >> 3] >> (r & 7) & 1) ? l : -INFINITY);
-                        }
+                        for (int r = 0; r < 8; ++r)
+                            if (__builtin_amdgcn_ballot_w64(counts[r] != 0)) l[r] = penalize(l[r], counts[r]);      // (most of a vocabulary is never seen)
                     }
-                    __builtin_amdgcn_sched_barrier(0);          // (one vector after the other: together they take more registers than there are)
+                    if (at.bias) l += at.bias_is_float ? load_eight(reinterpret_cast<const float*>(at.bias) + e) : load_eight(reinterpret_cast<const T*>(at.bias) + e);
+                    if (at.mask) {
+#pragma unroll
+                        for (int r = 0; r < 8; ++r) l[r] = allowed[q] & 1u << r ? l[r] : -INFINITY;
+                    }
+                    store_vec<O, 8>(at.out + e, __builtin_convertvector(l, vec<O, 8>));
+                } else {
+                    for (int r = e; r < n; ++r) {
+                        float l = (float)at.logits[r];
+                        if constexpr (HISTORY) l = penalize(l, seen[r]);
+                        if (at.bias) l += load_either<T>(at.bias, r, at.bias_is_float);
+                        at.out[r] = (O)(!at.mask || (at.mask[r >> 3] >> (r & 7) & 1) ? l : -INFINITY);
+                    }
                 }
+                __builtin_amdgcn_sched_barrier(0);          // (one vector after the other: together they take more registers than there are)
             }
         }
 }
@@ -174,11 +171,11 @@ template <typename T, typename O>
 hipError_t launch_typed(const dgnn_logits_args& a, hipStream_t stream)
 {
     const bool history = a.history && a.t > 0;
-    // two workgroups for every unit where there are tokens for that; threads for the chunk's vectors, and for a history that is longer
+    // two workgroups for every unit where there are tokens for that; threads that hold the chunk's vectors, more for a history that is longer
     int chunk = kMaxChunk;
     while (chunk > kMinChunk && a.b * ((a.v + chunk - 1) / chunk) < 512) chunk /= 2;
     int threads = power_of_two(history && a.t / 8 > chunk / (8 * kEach) ? a.t / 8 : chunk / (8 * kEach));
-    threads = threads < 64 ? 64 : threads > 1024 ? 1024 : threads;
+    threads = threads < 64 ? 64 : threads > kMaxThreads ? kMaxThreads : threads;
     const int chunks = (int)((a.v + chunk - 1) / chunk);
     const dim3 grid((unsigned)(chunks < (1 << 20) ? chunks : 1 << 20), (unsigned)(a.b < 65535 ? a.b : 65535));
     if (!history) return launch(logits_kernel<T, O, int32_t, false, false>, grid, dim3(threads), stream, a, chunk, chunks);
