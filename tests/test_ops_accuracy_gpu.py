@@ -97,6 +97,22 @@ def test_group_norm_with_all_the_lds_it_may_ask_for(ops, shape, groups, dtype):
     group_norm_case(ops, shape, groups, TYPES[dtype], "relu", affine=TYPES[dtype], residual=True, seed=groups)
 
 
+# ---- dense: the activations -----------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype,out", [("fp16", "fp32"), ("bf16", "fp32"), ("bf16", "bf16")])
+def test_gelu_keeps_its_digits(ops, dtype, out):
+    """x * 1 is exact, so what shows is the activation alone.  v Phi(v), with the tail Phi(-|v|) = exp(-v^2 / 2) P: the exponent is off by 2.5 half steps of its
+    size (the square, the factor log2(e) / 2 and the product with it), exp2 and the reciprocal by a step each, P and the products by 12 half steps, beside
+    2.5 of the polynomial itself; 1 - tail and the last product by 1.5."""
+    t = TYPES[dtype]
+    v = torch.cat([torch.linspace(-12.5, 12.5, 40001, dtype=torch.float64), torch.logspace(-6, 1, 4001, dtype=torch.float64), -torch.logspace(-6, 1, 4001, dtype=torch.float64)]).to(t)
+    y = ops.dense(v[:, None].cuda(), torch.ones(1, 1, dtype=t, device="cuda"), activation="gelu", out_dtype=TYPES[out])[:, 0]
+    d = v.double()
+    tail = 0.5 * torch.special.erfc(d.abs() / math.sqrt(2.0))
+    slack = ULP * d.abs() * (tail * (1.25 * d * d + 20) + torch.where(d < 0, tail * 0, 1.5 + tail * 0))
+    close(y, torch.where(d < 0, d * tail, d * (1 - tail)), slack, (dtype, out))
+
+
 # ---- logits -----------------------------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("b,v", [(3, 362), (5, 20011)])
