@@ -113,6 +113,18 @@ def test_gelu_keeps_its_digits(ops, dtype, out):
     close(y, torch.where(d < 0, d * tail, d * (1 - tail)), slack, (dtype, out))
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_tanh_keeps_its_digits(ops, dtype):
+    """Up to 0.7 an odd polynomial: the square, its products with the coefficients and the last two roundings, 3 half steps. Beyond, 1 - w with w = 2 / (exp(2 |x|) + 1):
+    w is off by 2 |x| half steps of the exponent, two each of exp2 and the reciprocal and one of the sum; the difference is what is rounded to the result."""
+    t = TYPES[dtype]
+    v = torch.cat([torch.linspace(-12, 12, 40001, dtype=torch.float64), torch.logspace(-6, 1, 4001, dtype=torch.float64), -torch.logspace(-6, 1, 4001, dtype=torch.float64)]).to(t)
+    y = ops.dense(v[:, None].cuda(), torch.ones(1, 1, dtype=t, device="cuda"), activation="tanh", out_dtype=torch.float32)[:, 0]
+    d = v.double()
+    w = 2 / (torch.exp(2 * d.abs()) + 1)
+    close(y, torch.tanh(d), ULP * torch.where(d.abs() < 0.7, 2 * d.abs(), w * (2 * d.abs() + 5)), dtype)
+
+
 # ---- logits -----------------------------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("b,v", [(3, 362), (5, 20011)])
