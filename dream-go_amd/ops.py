@@ -9,7 +9,7 @@
 The tensors are torch tensors on one GPU.  A call enqueues its work on the current torch stream of THAT device, whatever the current
 device is, and returns; it may be captured into a graph.  Errors are api.Error with the status codes of the C ABI; arguments are
 checked before anything is enqueued.  The operators evaluate and are not differentiable: a tensor that requires grad is refused while
-gradients are being recorded.  There is no CPU fallback.
+gradients are being recorded, and one with a forward-mode tangent always.  There is no CPU fallback.
 
 A predictor made of them goes behind the leaf pool and the search like any other (api.python_predictor).
 """
@@ -18,6 +18,7 @@ import os
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from . import api
 
@@ -103,16 +104,21 @@ def _first(where, name, t, types):
 
 
 def _records(*operands):
-    """Whether gradients are being recorded and one of the operands asks for its own."""
+    """Whether gradients are being recorded and one of the operands asks for its own, or one has a forward-mode tangent (those are carried on under
+    torch.no_grad() too)."""
     if torch.is_grad_enabled():
         for t in operands:
             if t is not None and t.requires_grad:
+                return True
+    if getattr(forward_ad, "_current_level", 0) >= 0:          # inside a dual_level
+        for t in operands:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
                 return True
     return False
 
 
 def _no_grad(where):
-    _refuse(where, "an operand requires grad: the operators evaluate only (torch.no_grad() or detach())", api.UNSUPPORTED)
+    _refuse(where, "an operand requires grad or has a tangent: the operators evaluate only (torch.no_grad(), detach(), unpack_dual().primal)", api.UNSUPPORTED)
 
 
 def _rows(where, name, t, rows, columns, broadcast=False):

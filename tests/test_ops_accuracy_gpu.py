@@ -141,3 +141,26 @@ def test_a_repetition_divides(ops, b, v):
     small = logits * 2.0 ** -100
     got = ops.adjust_logits(small.cuda(), history=history.cuda(), repetition=tiny.cuda()).cpu()
     assert torch.equal(got[small > 0], (small / tiny[:, None])[small > 0])
+
+
+# ---- what a call leaves behind, and what it refuses ---------------------------------------------------------------------------------------
+
+def test_forward_mode_tangents_are_refused(ops, api):
+    """A dual tensor does not ask for gradients; its tangent would be lost all the same."""
+    import torch.autograd.forward_ad as forward
+    h = torch.ones(4, 16, dtype=torch.float16, device="cuda")
+    maps, logits, history = h.view(2, 2, 16), h.float(), torch.zeros(4, 3, dtype=torch.int32, device="cuda")
+    with forward.dual_level():
+        def dual(t): return forward.make_dual(t, torch.ones_like(t))           # noqa: E306,E704
+        calls = [lambda: ops.dense(dual(h), h), lambda: ops.dense(h, dual(h)), lambda: ops.dense(h, h, dual(h[0, :4].contiguous())),
+                 lambda: ops.dense(h, h, residual=dual(h[:, :4].contiguous())), lambda: ops.group_norm(dual(maps), 4), lambda: ops.group_norm(maps, 4, dual(h[0])),
+                 lambda: ops.group_norm(maps, 4, residual=dual(maps)), lambda: ops.adjust_logits(dual(logits)), lambda: ops.adjust_logits(logits, bias=dual(logits)),
+                 lambda: ops.adjust_logits(logits, history=history, frequency=dual(logits[:, 0].contiguous()))]
+        for run in calls:
+            for mode in (torch.enable_grad, torch.no_grad):                    # (no_grad does not stop tangents: torch's own operators carry them on)
+                with mode(), pytest.raises(api.Error) as e:
+                    run()
+                assert e.value.status == api.UNSUPPORTED
+        assert ops.dense(h, h).shape == (4, 4)                                 # nothing here has a tangent
+        assert ops.dense(forward.unpack_dual(dual(h)).primal, h).shape == (4, 4)
+    assert ops.dense(h, h).shape == (4, 4)

@@ -175,3 +175,18 @@ def test_channels_are_counted_without_overflow(tmp_path):
     (tmp_path / "s.cpp").write_text('#include "ops.h"\n' + lines)
     subprocess.run(["g++", "-std=c++17", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include", "-I", os.path.join(ROOT, "dream-go_amd", "csrc"), "-fsyntax-only", str(tmp_path / "s.cpp")],
                    check=True)
+
+
+def test_what_carries_gradients_is_seen(ops):
+    import torch
+    import torch.autograd.forward_ad as forward
+    x, leaf = torch.ones(3), torch.ones(3, requires_grad=True)
+    assert ops._records(x, None, leaf) and not ops._records(x, None)
+    with torch.no_grad():
+        assert not ops._records(leaf)
+    with forward.dual_level():
+        dual = forward.make_dual(x, torch.ones(3))
+        assert ops._records(None, dual) and not ops._records(x, None)
+        with torch.no_grad():
+            assert ops._records(x, dual) and not ops._records(leaf, forward.unpack_dual(dual).primal)
+    assert not ops._records(x)
