@@ -9,7 +9,7 @@
 The tensors are torch tensors on one GPU.  A call enqueues its work on the current torch stream of THAT device, whatever the current
 device is, and returns; it may be captured into a graph.  Errors are api.Error with the status codes of the C ABI; arguments are
 checked before anything is enqueued.  The operators evaluate and are not differentiable: a tensor that requires grad is refused while
-gradients are being recorded, and one with a forward-mode tangent always.  There is no CPU fallback.
+gradients are being recorded, and one with a forward-mode tangent always.  An `out` counts as changed in place.  There is no CPU fallback.
 
 A predictor made of them goes behind the leaf pool and the search like any other (api.python_predictor).
 """
@@ -19,6 +19,7 @@ import struct
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from . import api
 
@@ -225,7 +226,8 @@ def dense(x, weight, bias=None, residual=None, *, alpha1=1.0, alpha2=1.0, activa
             _refuse(where, f"residual is {tuple(residual.shape)}, expected {(*leading, n)} or {(n,)}")
         else:
             ldz = n if residual.is_contiguous() else _rows(where, "residual", _flat(where, "residual", residual, m), m, n)
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty((*leading, n), dtype=out_dtype, device=x.device)
         py, ldy = out.data_ptr(), n
     else:
@@ -237,6 +239,8 @@ def dense(x, weight, bias=None, residual=None, *, alpha1=1.0, alpha2=1.0, activa
         _no_grad(where)
     _launch(where, lib.dgnn_dense, lib.dgnn_dense_workspace, index, _DENSE,
             (x.data_ptr(), pw, pb, pz, py, 0, 0, m, n, k, ldx, ldw, ldz, ldy, alpha1, alpha2, code, _TYPES[out_dtype], bias_code, _activation(where, activation)))
+    if given:
+        increment_version(out)      # what autograd has saved of it is not what it holds now
     return out
 
 
@@ -287,7 +291,8 @@ def group_norm(x, num_groups, weight=None, bias=None, residual=None, *, eps=1e-5
     if residual is not None:
         pz = _pointer(where, "residual", residual, index, (dtype,))
         z_n, z_p = (p * c, c) if residual.is_contiguous() and residual.shape == shape else _maps(where, "residual", residual, shape)
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty_like(x) if x.is_contiguous() else torch.empty(shape, dtype=dtype, device=x.device)
         py, y_n, y_p = out.data_ptr(), p * c, c
     else:
@@ -298,6 +303,8 @@ def group_norm(x, num_groups, weight=None, bias=None, residual=None, *, eps=1e-5
     _launch(where, lib.dgnn_group_norm, lib.dgnn_group_norm_workspace, index, _GROUP_NORM,
             (x.data_ptr(), pw, pb, pz, py, 0, 0, n, p, c, num_groups, x_n, x_p, z_n, z_p, y_n, y_p, eps, _TYPES[dtype], _TYPES[affine],
              _activation(where, activation)))
+    if given:
+        increment_version(out)      # what autograd has saved of it is not what it holds now
     return out
 
 
@@ -362,7 +369,8 @@ def adjust_logits(logits, *, mask=None, bias=None, history=None, lengths=None, p
             _vector(where, "prompt_lengths", prompt_lengths, b)
     elif lengths is not None or prompt_lengths is not None:
         _refuse(where, "lengths without history")
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty_like(logits) if logits.is_contiguous() else torch.empty((b, v), dtype=dtype, device=logits.device)
         po, ld_out, out_dtype = out.data_ptr(), v, dtype
     else:
@@ -373,4 +381,6 @@ def adjust_logits(logits, *, mask=None, bias=None, history=None, lengths=None, p
     _launch(where, lib.dgnn_adjust_logits, None, index, _LOGITS,
             (logits.data_ptr(), po, pm, pb, ph if t else 0, pn, pp, repetitions, presences, frequencies, b, v, t, ld_logits, ld_out, ld_mask, ld_bias, ld_history,
              repetition, presence, frequency, _TYPES[dtype], _TYPES[out_dtype], bias_code, history_code))
+    if given:
+        increment_version(out)      # what autograd has saved of it is not what it holds now
     return out

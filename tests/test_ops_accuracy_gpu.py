@@ -164,3 +164,20 @@ def test_forward_mode_tangents_are_refused(ops, api):
         assert ops.dense(h, h).shape == (4, 4)                                 # nothing here has a tangent
         assert ops.dense(forward.unpack_dual(dual(h)).primal, h).shape == (4, 4)
     assert ops.dense(h, h).shape == (4, 4)
+
+
+def test_a_result_written_over_a_saved_tensor_is_noticed(ops):
+    """What autograd keeps for a backward pass and an operator then writes over: the backward pass says so, as behind torch's own operators."""
+    h = torch.ones(4, 4, dtype=torch.float16, device="cuda")
+    maps = torch.ones(2, 2, 4, device="cuda")
+    logits = torch.ones(4, 4, device="cuda")
+    for out, run in ((h.clone(), lambda o: ops.dense(h, h, out=o)), (maps.clone(), lambda o: ops.group_norm(maps, 2, out=o)), (logits.clone(), lambda o: ops.adjust_logits(logits, out=o))):
+        leaf = torch.ones_like(out, requires_grad=True)
+        loss = (leaf * out).sum()
+        before = out._version
+        assert run(out) is out and out._version > before
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    with torch.inference_mode():
+        buffer = torch.empty(4, 4, dtype=torch.float16, device="cuda")
+        assert ops.dense(h, h, out=buffer) is buffer
