@@ -14,6 +14,7 @@ gradients are being recorded, and one with a forward-mode tangent always.  An `o
 A predictor made of them goes behind the leaf pool and the search like any other (api.python_predictor).
 """
 import ctypes
+import operator
 import os
 import struct
 
@@ -111,7 +112,7 @@ def _records(*operands):
         for t in operands:
             if t is not None and t.requires_grad:
                 return True
-    if getattr(forward_ad, "_current_level", 0) >= 0:          # inside a dual_level
+    if forward_ad._current_level >= 0:                          # inside a dual_level
         for t in operands:
             if t is not None and forward_ad.unpack_dual(t).tangent is not None:
                 return True
@@ -153,6 +154,18 @@ def _flat(where, name, t, leading):
         _refuse(where, f"{name}'s leading dimensions do not make rows of one stride", api.UNSUPPORTED)
 
 
+def _number(where, name, value):
+    """A number as the block takes it (rounded to fp32 there).  Of a tensor it is the value, so one that carries gradients is refused."""
+    if isinstance(value, torch.Tensor) and _records(value):
+        _no_grad(where)
+    try:
+        if isinstance(value, (str, bytes)):
+            raise TypeError
+        return float(value)
+    except (TypeError, ValueError, OverflowError, RuntimeError):               # (RuntimeError: a tensor of more than one element)
+        _refuse(where, f"{name} must be a number, got {type(value).__name__}")
+
+
 def _activation(where, name):
     code = ACTIVATIONS.get(name)
     if code is None:
@@ -170,13 +183,16 @@ def _stream(index):
 
 def _launch(where, run, workspace, index, block, args):
     """One call; once more with work memory where it asks for some."""
+    try:
+        packed = block.pack(*args)
+    except struct.error as error:
+        _refuse(where, f"an argument is out of its type's range ({error})")
     stream = _stream(index)
-    status = run(index, stream, block.pack(*args))
+    status = run(index, stream, packed)
     if status == 0:
         return
     if status == api.BAD_ARGUMENT and workspace is not None:
         need = ctypes.c_int64()
-        packed = block.pack(*args)
         if workspace(packed, need) == 0 and need.value:
             memory = torch.empty(need.value, dtype=torch.uint8, device=torch.device("cuda", index))
             status = run(index, stream, block.pack(*args[:5], memory.data_ptr(), need.value, *args[7:]))
@@ -237,6 +253,8 @@ def dense(x, weight, bias=None, residual=None, *, alpha1=1.0, alpha2=1.0, activa
         ldy = n if out.is_contiguous() else _rows(where, "out", _flat(where, "out", out, m), m, n)
     if _records(x, weight, bias, residual, out):
         _no_grad(where)
+    if type(alpha1) is not float or type(alpha2) is not float:
+        alpha1, alpha2 = _number(where, "alpha1", alpha1), _number(where, "alpha2", alpha2)
     _launch(where, lib.dgnn_dense, lib.dgnn_dense_workspace, index, _DENSE,
             (x.data_ptr(), pw, pb, pz, py, 0, 0, m, n, k, ldx, ldw, ldz, ldy, alpha1, alpha2, code, _TYPES[out_dtype], bias_code, _activation(where, activation)))
     if given:
@@ -276,6 +294,11 @@ def group_norm(x, num_groups, weight=None, bias=None, residual=None, *, eps=1e-5
     n, c = shape[0], shape[-1]
     p = shape[1] if len(shape) == 3 else shape[1:-1].numel()
     x_n, x_p = (p * c, c) if x.is_contiguous() else _maps(where, "x", x, shape)
+    if type(num_groups) is not int:
+        try:
+            num_groups = operator.index(num_groups)
+        except TypeError:
+            _refuse(where, f"num_groups must be a whole number, got {type(num_groups).__name__}")
     if num_groups < 1 or c % num_groups:
         _refuse(where, f"{num_groups} groups do not divide {c} channels")
     pw = pb = pz = z_n = z_p = 0
@@ -301,7 +324,7 @@ def group_norm(x, num_groups, weight=None, bias=None, residual=None, *, eps=1e-5
     if _records(x, weight, bias, residual, out):
         _no_grad(where)
     _launch(where, lib.dgnn_group_norm, lib.dgnn_group_norm_workspace, index, _GROUP_NORM,
-            (x.data_ptr(), pw, pb, pz, py, 0, 0, n, p, c, num_groups, x_n, x_p, z_n, z_p, y_n, y_p, eps, _TYPES[dtype], _TYPES[affine],
+            (x.data_ptr(), pw, pb, pz, py, 0, 0, n, p, c, num_groups, x_n, x_p, z_n, z_p, y_n, y_p, eps if type(eps) is float else _number(where, "eps", eps), _TYPES[dtype], _TYPES[affine],
              _activation(where, activation)))
     if given:
         increment_version(out)      # what autograd has saved of it is not what it holds now
@@ -314,7 +337,7 @@ def _per_row(where, name, value, index, rows):
         p = _pointer(where, name, value, index, (torch.float32,))
         _vector(where, name, value, rows)
         return p, 1.0
-    return 0, float(value)
+    return 0, value if type(value) is float else _number(where, name, value)
 
 
 def adjust_logits(logits, *, mask=None, bias=None, history=None, lengths=None, prompt_lengths=None,

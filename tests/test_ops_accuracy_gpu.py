@@ -181,3 +181,20 @@ def test_a_result_written_over_a_saved_tensor_is_noticed(ops):
     with torch.inference_mode():
         buffer = torch.empty(4, 4, dtype=torch.float16, device="cuda")
         assert ops.dense(h, h, out=buffer) is buffer
+
+
+def test_numbers_that_are_none_are_refused(ops, api):
+    h = torch.ones(4, 16, dtype=torch.float16, device="cuda")
+    maps, logits, history = h.view(2, 2, 16), h.float(), torch.zeros(4, 3, dtype=torch.int32, device="cuda")
+    learned = torch.tensor(0.5, device="cuda", requires_grad=True)
+    bad = [lambda: ops.dense(h, h, alpha2="2"), lambda: ops.dense(h, h, alpha1=None), lambda: ops.dense(h, h, alpha1=learned),
+           lambda: ops.dense(h, h, residual=h[:, :4].contiguous(), alpha2=learned), lambda: ops.group_norm(maps, 4, eps=1e39), lambda: ops.group_norm(maps, 4, eps=None),
+           lambda: ops.group_norm(maps, 4, eps=learned), lambda: ops.group_norm(maps, 4.0), lambda: ops.group_norm(maps, None), lambda: ops.group_norm(maps[..., :0], 1 << 70),
+           lambda: ops.adjust_logits(logits, repetition=1e39), lambda: ops.adjust_logits(logits, history=history, presence=None),
+           lambda: ops.adjust_logits(logits, history=history, frequency="much"), lambda: ops.adjust_logits(logits, history=history, frequency=learned)]
+    for n, run in enumerate(bad):
+        with pytest.raises(api.Error) as e:
+            run()
+        assert e.value.status in (api.BAD_ARGUMENT, api.UNSUPPORTED), n
+    with torch.no_grad():
+        assert torch.equal(ops.dense(h, h, alpha1=learned), ops.dense(h, h, alpha1=0.5))

@@ -190,3 +190,19 @@ def test_what_carries_gradients_is_seen(ops):
         with torch.no_grad():
             assert ops._records(x, dual) and not ops._records(leaf, forward.unpack_dual(dual).primal)
     assert not ops._records(x)
+
+
+def test_numbers(ops, api):
+    import torch
+    learned = torch.tensor(0.5, requires_grad=True)
+    for bad in (None, "1", b"1", 1j, [1.0], {}, 1 << 2000, torch.ones(2), learned):
+        with pytest.raises(api.Error) as e:
+            ops._number("dense", "alpha1", bad)
+        assert e.value.status == (api.UNSUPPORTED if bad is learned else api.BAD_ARGUMENT) and str(e.value).count("dense")
+    for good in (0, 2, True, 0.5, np.float32(0.5), np.int64(3), torch.tensor(0.5), learned.detach()):
+        assert ops._number("dense", "alpha1", good) == float(good)
+    with torch.no_grad():
+        assert ops._number("dense", "alpha1", learned) == 0.5
+    with pytest.raises(api.Error) as e:
+        ops._launch("group_norm", None, None, 0, ops._GROUP_NORM, [0] * 11 + [1 << 70] + [0] * 6 + [1.0] + [0] * 3)
+    assert e.value.status == api.BAD_ARGUMENT
