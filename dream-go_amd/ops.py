@@ -167,7 +167,7 @@ def _number(where, name, value):
 
 
 def _activation(where, name):
-    code = ACTIVATIONS.get(name)
+    code = ACTIVATIONS.get(name) if isinstance(name, str) else None
     if code is None:
         _refuse(where, f"activation {name!r} is none of {', '.join(ACTIVATIONS)}")
     return code
@@ -225,7 +225,7 @@ def dense(x, weight, bias=None, residual=None, *, alpha1=1.0, alpha2=1.0, activa
     ldx = k if x.is_contiguous() else _rows(where, "x", _flat(where, "x", x, m), m, k)
     ldw = k if weight.is_contiguous() else _rows(where, "weight", weight, n, k)
     if out_dtype is None:
-        out_dtype = dtype if out is None else out.dtype
+        out_dtype = dtype if not isinstance(out, torch.Tensor) else out.dtype
     if out_dtype is not dtype and out_dtype is not torch.float32:
         _refuse(where, f"out_dtype {out_dtype} is neither x's type nor torch.float32", api.UNSUPPORTED)
     pb = pz = ldz = 0

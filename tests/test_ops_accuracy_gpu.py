@@ -198,3 +198,15 @@ def test_numbers_that_are_none_are_refused(ops, api):
         assert e.value.status in (api.BAD_ARGUMENT, api.UNSUPPORTED), n
     with torch.no_grad():
         assert torch.equal(ops.dense(h, h, alpha1=learned), ops.dense(h, h, alpha1=0.5))
+
+
+def test_operands_that_are_no_tensors_are_refused(ops, api):
+    h, f = torch.ones(4, 16, dtype=torch.float16, device="cuda"), torch.ones(4, 16, device="cuda")
+    bad = [lambda: ops.dense(h, h, out=5), lambda: ops.dense(h, h, out=h.cpu().numpy()), lambda: ops.dense(h, h, activation=["relu"]), lambda: ops.dense([h], h),
+           lambda: ops.dense(h, h, out_dtype="fp16"), lambda: ops.dense(h, None), lambda: ops.dense(h, h, residual=0.0), lambda: ops.group_norm(f, 4, out=5),
+           lambda: ops.group_norm(f, 4, 1.0), lambda: ops.group_norm(f, 4, activation={}), lambda: ops.adjust_logits(f, out=5), lambda: ops.adjust_logits(f, mask=[1]),
+           lambda: ops.adjust_logits(f, bias=1.0), lambda: ops.adjust_logits(f, history=[[1]]), lambda: ops.adjust_logits(f, history=torch.zeros(4, 1, dtype=torch.int32, device="cuda"), lengths=1)]
+    for n, run in enumerate(bad):
+        with pytest.raises(api.Error) as e:
+            run()
+        assert e.value.status in (api.BAD_ARGUMENT, api.UNSUPPORTED), n
