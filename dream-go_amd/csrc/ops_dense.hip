@@ -4,9 +4,10 @@
 // consecutive outputs n of one row m in a lane's four registers, which is how y lies in memory.  Sums are fp32; alpha1, z, bias and the
 // activation are applied in fp32 and the result is rounded once.
 //
-// Measured: 8192 x 16384 -> 4096 bf16 with a skip 872 us, 1261 TFLOP/s (bound by the matrix pipe under its power limit); 16 x 4096 -> 16384 26 us
+// Measured: 8192 x 16384 -> 4096 bf16 with a skip 868 us, 1267 TFLOP/s (bound by the matrix pipe under its power limit); 16 x 4096 -> 16384 26 us
 // (31 with the weights out of every cache: HBM, 4.3 TB/s); 1021 x 2027 -> 1531, where no row is aligned, 28 us, 9 of them the copies (then bound by a
-// unit's path to the L2); 256 x 2888 -> 362 fp16 10.8 us and one row of it 7.0 (chains of waits).
+// unit's path to the L2); 256 x 2888 -> 362 fp16 10.8 us and one row of it 6.9 (chains of waits); 2048 x
+// 4096 -> 4096 74 us, 928 TFLOP/s, and 512 rows of it 26.6 (tiles that do not come out even on 256 units).
 #include "ops_device.h"
 
 namespace dgnn {
@@ -237,7 +238,7 @@ struct Tile {
         else f.w[r == 0 ? 0 : r - FM] = *reinterpret_cast<const Frag*>(at + read_w + (r == 0 ? 0 : r - FM) * 16 * BK);
     }
 
-    // The products of one step; beside them the fragments of the next step are read and, with LOAD, the tile two ahead is asked for.  Nothing in
+    // The products of one step; beside them the fragments of the next step are read and, with LOAD, the tile S ahead is asked for.  Nothing in
     // here branches: the compiler keeps the sums and the fragments where they are.
     template <bool LOAD>
     __device__ __forceinline__ void step(floatx4 (&acc)[FN][FM], const Frags& f, Frags& next, int read_buffer, int read_step, int load_buffer, const char* w, const char* x)
@@ -458,7 +459,9 @@ void dense_pack_kernel(Packing w, Packing x, int64_t k, int64_t pitch, int lanes
 //
 // Where one of the operands has few rows, or both are small, there is little to share through LDS: a workgroup owns 16 x 16 outputs, its waves
 // share the columns of k in contiguous pieces and fetch the fragments they multiply, and their sums meet in LDS, in order.  Rows need no alignment.
-// Bound by what a unit's L1 passes on: 28 GB/s a unit at 16 x 8192 x 512 (18 us on 32 units), 5.2 TB/s of HBM at 1 x 4096 x 16384 (25.8 us).
+// Bound by what a unit's L1 passes on: 28 GB/s a unit at 16 x 8192 x 512 (18 us on 32 units); at 1 x 4096 x 16384 by HBM, 4.9 TB/s (27.5 us with the
+// weights out of every cache).  A wave with fewer than kUnroll steps takes them one by one, each load waited for before the next: 1 x 2888 x 362, six steps
+// a wave, spends most of its 6.9 us so.
 constexpr int kDirectWaves = 16;
 template <typename T>
 __global__ __launch_bounds__(kDirectWaves * 64)

@@ -11,7 +11,8 @@ device is, and returns; it may be captured into a graph.  Errors are api.Error w
 checked before anything is enqueued.  The operators evaluate and are not differentiable: a tensor that requires grad is refused while
 gradients are being recorded, and one with a forward-mode tangent always.  An `out` counts as changed in place.  There is no CPU fallback.
 
-A predictor made of them goes behind the leaf pool and the search like any other (api.python_predictor).
+A predictor made of them goes behind the leaf pool and the search like any other (api.python_predictor): that boundary is host memory, so the
+planes are copied to the device and value and policy back.
 """
 import ctypes
 import operator
