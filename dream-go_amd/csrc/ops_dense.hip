@@ -6,8 +6,8 @@
 //
 // Measured: 8192 x 16384 -> 4096 bf16 with a skip 868 us, 1267 TFLOP/s (bound by the matrix pipe under its power limit); 16 x 4096 -> 16384 26 us
 // (31 with the weights out of every cache: HBM, 4.3 TB/s); 1021 x 2027 -> 1531, where no row is aligned, 28 us, 9 of them the copies (then bound by a
-// unit's path to the L2); 256 x 2888 -> 362 fp16 10.8 us and one row of it 6.9 (chains of waits); 2048 x
-// 4096 -> 4096 74 us, 928 TFLOP/s, and 512 rows of it 26.6 (tiles that do not come out even on 256 units).
+// unit's path to the L2); 256 x 2888 -> 362 fp16 10.8 us and one row of it 6.9 (chains of waits);
+// 2048 x 4096 -> 4096 74 us, 928 TFLOP/s, and 512 rows of it 26.6 (tiles that do not come out even on 256 units).
 #include "ops_device.h"
 
 namespace dgnn {
@@ -68,7 +68,7 @@ __device__ __forceinline__ void finish_as(const dgnn_dense_args& a, int64_t m, i
                 for (int r = 0; r < 8; ++r) v[r] += (float)s[r];
             }
         }
-        activate(v, a.activation);
+        activate<O>(v, a.activation);
         vec<O, 8> out;
 #pragma unroll
         for (int r = 0; r < 8; ++r) out[r] = (O)v[r];
@@ -81,7 +81,7 @@ __device__ __forceinline__ void finish_as(const dgnn_dense_args& a, int64_t m, i
             if (z) v[r] = __builtin_fmaf(a.alpha2, (float)z[r], v[r]);
             if (a.bias) v[r] += load_either<T>(a.bias, n + r, bias_is_float);
         }
-        activate(v, a.activation);
+        activate<O>(v, a.activation);
 #pragma unroll
         for (int r = 0; r < 7; ++r)
             if (r < left) y[r] = (O)v[r];

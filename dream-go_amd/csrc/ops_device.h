@@ -49,7 +49,8 @@ __device__ __forceinline__ float exponential(float v) { return __builtin_amdgcn_
 //   gelu  v * Phi(v); Phi(-x) exp(x^2 / 2) is a polynomial of t = 1 / (1 + 0.3 x), fitted to it over 0 <= x <= 14 by least squares weighted for the
 //         smallest largest relative error, 1.5e-7.  The tail is the product itself, not 1 - erf: below zero it keeps its digits (the exponent's own
 //         rounding, x^2 / 2 times a few steps, is what it loses), and results are within 1.2e-7 of max(1, |v|) as measured on a grid
-//   silu  v times the reciprocal of 1 + exp(-v): within 1.5e-7 of max(1, |v|) on a grid, a division would be within 1.2e-7
+//   silu  v / (1 + exp(-v)), the quotient corrected to the last bit where the result stays fp32 (1.2e-7 of max(1, |v|) on a grid; fixup: where an infinity is
+//         divided or divides); the product with the reciprocal alone, 1.4e-7, where it is rounded to sixteen bits, whose half step is 4e3 times that
 __device__ __forceinline__ float tanh_of(float v)
 {
     const float q = v * v, x = __builtin_fabsf(v);
@@ -66,15 +67,23 @@ __device__ __forceinline__ float gelu_of(float v)
     const float tail = p * __builtin_amdgcn_exp2f(x * x * -0.72134752044448170f);           // Phi(-|v|)
     return v * (v < 0.0f ? tail : 1.0f - tail);
 }
-__device__ __forceinline__ float silu_of(float v) { return v * rcp(1.0f + exponential(-v)); }
+template <typename O>
+__device__ __forceinline__ float silu_of(float v)
+{
+    const float d = 1.0f + exponential(-v), r = rcp(d), q = v * r;
+    if constexpr (!__is_same(O, float)) return q;
+    else return __builtin_amdgcn_div_fixupf(__builtin_fmaf(__builtin_fmaf(-q, d, v), r, q), d, v);
+}
 
+// O: what the result is rounded to.
+template <typename O>
 __device__ __forceinline__ float activate(float v, int activation)
 {
     switch (activation) {
     case DGNN_ACT_RELU: return v < 0.0f ? 0.0f : v;
     case DGNN_ACT_TANH: return tanh_of(v);
     case DGNN_ACT_GELU: return gelu_of(v);
-    case DGNN_ACT_SILU: return silu_of(v);
+    case DGNN_ACT_SILU: return silu_of<O>(v);
     default: return v;
     }
 }
@@ -83,36 +92,36 @@ __device__ __forceinline__ float activate(float v, int activation)
 enum Kind { kPlain, kSilu, kAny };              // identity and ReLU; SiLU; every one
 
 // One branch for several values.
-template <int N>
+template <typename O, int N>
 __device__ __forceinline__ void activate(float (&v)[N], int activation)
 {
     switch (activation) {
     case DGNN_ACT_IDENTITY: break;
     case DGNN_ACT_RELU:
 #pragma unroll
-        for (int r = 0; r < N; ++r) v[r] = activate(v[r], DGNN_ACT_RELU);
+        for (int r = 0; r < N; ++r) v[r] = activate<O>(v[r], DGNN_ACT_RELU);
         break;
     case DGNN_ACT_TANH:
 #pragma unroll
-        for (int r = 0; r < N; ++r) v[r] = activate(v[r], DGNN_ACT_TANH);
+        for (int r = 0; r < N; ++r) v[r] = activate<O>(v[r], DGNN_ACT_TANH);
         break;
     case DGNN_ACT_GELU:
 #pragma unroll
-        for (int r = 0; r < N; ++r) v[r] = activate(v[r], DGNN_ACT_GELU);
+        for (int r = 0; r < N; ++r) v[r] = activate<O>(v[r], DGNN_ACT_GELU);
         break;
     default:
 #pragma unroll
-        for (int r = 0; r < N; ++r) v[r] = activate(v[r], DGNN_ACT_SILU);
+        for (int r = 0; r < N; ++r) v[r] = activate<O>(v[r], DGNN_ACT_SILU);
     }
 }
 
-template <Kind K, int N>
+template <Kind K, typename O, int N>
 __device__ __forceinline__ void activate_kind(float (&v)[N], int activation)
 {
-    if constexpr (K == kAny) activate(v, activation);
+    if constexpr (K == kAny) activate<O>(v, activation);
     else {
 #pragma unroll
-        for (int r = 0; r < N; ++r) v[r] = K == kSilu ? silu_of(v[r]) : activation == DGNN_ACT_RELU && v[r] < 0.0f ? 0.0f : v[r];
+        for (int r = 0; r < N; ++r) v[r] = K == kSilu ? silu_of<O>(v[r]) : activation == DGNN_ACT_RELU && v[r] < 0.0f ? 0.0f : v[r];
     }
 }
 

@@ -289,7 +289,7 @@ void one_pass_kernel(dgnn_group_norm_args a, Layout l)
                         v[e] = __builtin_fmaf((float)held[r][e] - mean[e], scale[e], bias[e]);
                         if constexpr (SKIP) v[e] += (float)skip[r][e];
                     }
-                    activate_kind<K>(v, a.activation);
+                    activate_kind<K, T>(v, a.activation);
                     store_part<S, T, V>(y, p.n, v);
                     y += l.rows * a.y_p;
                 }
@@ -491,7 +491,7 @@ void apply_kernel(dgnn_group_norm_args a, Layout l, const Moments* moments)
                             v[e] = __builtin_fmaf((float)held[r][e] - of_mean[e], scale[e], bias[e]);
                             if constexpr (SKIP) v[e] += (float)skip[r][e];
                         }
-                        activate_kind<K>(v, a.activation);
+                        activate_kind<K, T>(v, a.activation);
                         store_part<S, T, V>(y, p.n, v);
                         y += l.rows * a.y_p;
                     }

@@ -125,6 +125,26 @@ def test_tanh_keeps_its_digits(ops, dtype):
     close(y, torch.tanh(d), ULP * torch.where(d.abs() < 0.7, 2 * d.abs(), w * (2 * d.abs() + 5)), dtype)
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_silu_keeps_its_digits(ops, dtype):
+    """v / d with d = 1 + exp(-v) = 1 + exp2(v log2(e)): the exponent is off by one half step of its size for the product and by 0.23 of one for the factor, whose
+    nearest number of fp32 is 1.93e-8 below 1.442695, a relative 1.34e-8 = 0.23 * 2^-24; exp2 by a step.  Of d that is the part 1 - 1 / d; the sum is rounded once,
+    and the quotient once, which is the result's own rounding."""
+    t = TYPES[dtype]
+    v = torch.cat([torch.linspace(-60, 60, 40001, dtype=torch.float64), torch.logspace(-6, 1, 4001, dtype=torch.float64), -torch.logspace(-6, 1, 4001, dtype=torch.float64)]).to(t)
+    one = torch.ones(1, 1, dtype=t, device="cuda")
+    y = ops.dense(v[:, None].cuda(), one, activation="silu", out_dtype=torch.float32)[:, 0]
+    d = v.double()
+    ref, part = d / (1 + torch.exp(-d)), 1 - 1 / (1 + torch.exp(-d))
+    close(y, ref, ULP * ref.abs() * (part * (1.23 * d.abs() + 2.5) + 1), dtype)
+    # as 16 bits, and of infinities: v / (1 + exp(-v)) is infinite, and of minus infinity no number
+    assert torch.equal(ops.dense(v[:, None].cuda(), one, activation="silu")[:, 0].isnan().cpu(), v.isnan())
+    x = torch.tensor([[math.inf], [-math.inf], [math.nan], [100.0], [-100.0], [0.0], [-3e4]], dtype=t, device="cuda")
+    for out in (torch.float32, t):
+        got = ops.dense(x, one, activation="silu", out_dtype=out)[:, 0].float().cpu()
+        assert got[0] == math.inf and got[1].isnan() and got[2].isnan() and got[3] == 100 and (got[4:].abs() < 1e-30).all(), got
+
+
 # ---- logits -----------------------------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("b,v", [(3, 362), (5, 20011)])
